@@ -45,6 +45,11 @@ EXPORTED_SYMBOLS = (
     "b200attn_ipc_open",
     "b200attn_ipc_close",
     "b200attn_copy_async",
+    "b200attn_plan_create",
+    "b200attn_plan_table",
+    "b200attn_plan_destroy",
+    "b200attn_forward_planned",
+    "b200attn_qk_norm_rope",
     "b200attn_status_string",
     "b200attn_last_error",
     "b200attn_version",
@@ -93,6 +98,95 @@ class ForwardArgs(C.Structure):
     ]
 
 
+class PlanDesc(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_uint32),
+        ("sequences", C.c_int32),
+        ("heads", C.c_int32),
+        ("heads_kv", C.c_int32),
+        ("causal", C.c_int32),
+        ("len_prefix", C.c_int32),
+        ("sm_count", C.c_int32),
+        ("reserved", C.c_int32),
+        ("len_q", C.POINTER(C.c_int32)),
+        ("len_kv", C.POINTER(C.c_int32)),
+        ("start_kv", C.POINTER(C.c_int64)),
+    ]
+
+
+class PlanInfo(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_uint32),
+        ("grid", C.c_int32),
+        ("pieces", C.c_int32),
+        ("units", C.c_int32),
+        ("rows_q", C.c_int64),
+        ("rows_kv", C.c_int64),
+        ("slot_rows", C.c_int64),
+        ("table_bytes", C.c_uint64),
+        ("workspace_bytes", C.c_uint64),
+    ]
+
+
+class PlannedArgs(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_uint32),
+        ("heads", C.c_int32),
+        ("heads_kv", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("rows_q", C.c_int32),
+        ("rows_kv", C.c_int32),
+        ("len_prefix", C.c_int32),
+        ("grid", C.c_int32),
+        ("join_units", C.c_int32),
+        ("reserved", C.c_int32),
+        ("q", Operand),
+        ("k", Operand),
+        ("v", Operand),
+        ("k_prefix", Operand),
+        ("v_prefix", Operand),
+        ("o", Operand),
+        ("lse", C.c_void_p),
+        ("lse_stride_head", C.c_int64),
+        ("softmax_scale", C.c_float),
+        ("reserved2", C.c_int32),
+        ("table", C.c_void_p),
+        ("workspace", C.c_void_p),
+        ("slot_rows", C.c_int64),
+        ("stream", C.c_void_p),
+    ]
+
+
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [
+        ("struct_bytes", C.c_uint32),
+        ("batch", C.c_int32),
+        ("tokens", C.c_int32),
+        ("heads_q", C.c_int32),
+        ("heads_k", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("q", Operand),
+        ("k", Operand),
+        ("q_out", Operand),
+        ("k_out", Operand),
+        ("q_weight", C.c_void_p),
+        ("k_weight", C.c_void_p),
+        ("weight_type", C.c_int32),
+        ("position_type", C.c_int32),
+        ("positions", C.c_void_p),
+        ("position_stride_axis", C.c_int64),
+        ("position_stride_batch", C.c_int64),
+        ("position_stride_token", C.c_int64),
+        ("inv_freq", C.c_void_p),
+        ("axes", C.c_int32),
+        ("section", C.c_int32 * 4),
+        ("eps", C.c_float),
+        ("interleaved", C.c_int32),
+        ("reserved", C.c_int32),
+        ("stream", C.c_void_p),
+    ]
+
+
 _lib = None
 
 
@@ -134,6 +228,16 @@ def lib() -> C.CDLL:
         handle.b200attn_ipc_close.restype = C.c_int
         handle.b200attn_copy_async.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]
         handle.b200attn_copy_async.restype = C.c_int
+        handle.b200attn_plan_create.argtypes = [C.POINTER(PlanDesc), C.POINTER(PlanInfo), C.POINTER(C.c_void_p)]
+        handle.b200attn_plan_create.restype = C.c_int
+        handle.b200attn_plan_table.argtypes = [C.c_void_p, C.c_void_p, C.c_uint64]
+        handle.b200attn_plan_table.restype = C.c_int
+        handle.b200attn_plan_destroy.argtypes = [C.c_void_p]
+        handle.b200attn_plan_destroy.restype = C.c_int
+        handle.b200attn_forward_planned.argtypes = [C.POINTER(PlannedArgs)]
+        handle.b200attn_forward_planned.restype = C.c_int
+        handle.b200attn_qk_norm_rope.argtypes = [C.POINTER(QkNormRopeArgs)]
+        handle.b200attn_qk_norm_rope.restype = C.c_int
         handle.b200attn_status_string.argtypes = [C.c_int]
         handle.b200attn_status_string.restype = C.c_char_p
         handle.b200attn_last_error.argtypes = []

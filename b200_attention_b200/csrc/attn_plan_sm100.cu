@@ -1,0 +1,685 @@
+// Planned attention for sm_100a: packed sequences of different lengths, grouped heads, causal masks, and
+// requests that share a prefix, in one persistent kernel that walks a schedule made on the host
+// (plan.cpp), and a second small kernel that joins partial results.
+//
+//   O_i = sum_j p_ij V_j,  p_ij = 2^(c s_ij - m_i) / sum_j 2^(c s_ij - m_i),  s = Q K^T,  c = scale * log2(e)
+//   joining two runs of keys a and b of a row:  lse = log(e^lse_a + e^lse_b),
+//   O = O_a e^(lse_a - lse) + O_b e^(lse_b - lse)
+//
+// The kernel is built like attn_fwd_ws_kernel (same tiles, descriptors, TMEM layout and softmax):
+//   warps 0-3, 4-7  softmax of Q tile 0 / 1, a row per thread
+//   warps 8-11      epilogue: bf16 O and LSE, or an fp32 partial
+//   warp 12         tcgen05.mma     warp 13  TMA loads
+//   warp 14         clears the rows of a V tile behind the last key: they belong to another sequence or to
+//                   memory nobody wrote, and 0 * NaN is NaN in the product P V
+// What differs is where work comes from. Query heads that share a K/V head are packed into the rows of a
+// tile (row = token * group + head of the group, which is one TMA box of floor(128 / group) tokens x group
+// heads), so a K/V tile is read once for the whole group, a single token fills `group` rows instead of one,
+// and a block of rows spans fewer tokens and so fewer tiles that the causal diagonal cuts.
+
+#include "attn_device_sm100.cuh"
+#include "plan_kernels.cuh"
+
+namespace b200attn {
+
+namespace {
+
+constexpr int kPairSlotsP = 2;
+constexpr int kPairBytesP = 2 * kTileBytes;
+constexpr int kPlanThreads = 512;
+constexpr int kPlanRegsSoftmax = 192;
+constexpr int kPlanRegsEpilogue = 64;
+constexpr int kPlanRegsOther = 64;
+constexpr int kPieceCache = 192;  // pieces of a CTA kept in shared memory; further ones are read from the table
+
+enum PlanBarrier : int {
+  kPbQFull = 0,      // +q    TMA -> MMA
+  kPbQEmpty = 2,     // +q    MMA -> TMA
+  kPbSFull = 4,      // +q    MMA -> softmax
+  kPbPReady = 6,     // +q    softmax (4 warps) -> MMA
+  kPbPvDone = 8,     // +q    MMA -> epilogue
+  kPbFin = 10,       // +q    softmax (4 warps) -> epilogue
+  kPbFinFree = 12,   // +q    epilogue (4 warps) -> softmax
+  kPbOFree = 14,     // +q    epilogue (4 warps) -> MMA
+  kPbPairFull = 16,  // +slot TMA -> MMA, warp 14
+  kPbPairEmpty = 18, // +slot MMA and warp 14 -> TMA
+  kPbTailClean = 20, //       warp 14 -> MMA: the rows of a V tile behind the last key are zero
+  kPbDrain = 21,
+  kNumPlanBarriers = 22
+};
+
+struct alignas(16) PlanAux {
+  uint64_t bar[kNumPlanBarriers];
+  float row_max[kQTilesPerItem][kBlockM];
+  float row_sum[kQTilesPerItem][kBlockM];
+  uint32_t tmem_base;
+  uint32_t abort_flag;
+  int32_t piece0, piece1;
+  PlanPiece cache[kPieceCache];
+};
+
+constexpr int kPlanSmemBytes = kQTilesPerItem * kTileBytes + kPairSlotsP * kPairBytesP + int(sizeof(PlanAux));
+static_assert(kPlanSmemBytes <= 227 * 1024, "shared memory of a CTA");
+
+// Every role walks the CTA's pieces in the same order.
+struct PlanWalk {
+  const PlanAux* aux;
+  const PlanPiece* table;
+  int i, n;
+  __device__ __forceinline__ PlanWalk(const PlanParams& p, const PlanAux* a)
+      : aux(a), table(reinterpret_cast<const PlanPiece*>(p.table + kPlanPieceAt) + a->piece0), i(0),
+        n(a->piece1 - a->piece0) {}
+  __device__ __forceinline__ bool take(const PlanPiece*& out) {
+    if (i >= n) return false;
+    out = i < kPieceCache ? &aux->cache[i] : table + i;
+    ++i;
+    return true;
+  }
+  __device__ __forceinline__ const PlanPiece* peek() const {
+    return i >= n ? nullptr : (i < kPieceCache ? &aux->cache[i] : table + i);
+  }
+};
+
+__device__ __forceinline__ int piece_tiles(const PlanPiece* pc) { return max(pc->tiles[0], pc->tiles[1]); }
+
+// Keys in the last tile that the piece visits, if its keys end inside it; 0 otherwise.
+__device__ __forceinline__ int piece_tail(const PlanPiece* pc) {
+  const int in_last = pc->n_keys - (piece_tiles(pc) - 1) * kBlockN;
+  return in_last < kBlockN ? in_last : 0;
+}
+
+// ---- TMA producer: K/V in pairs (V of one tile, K of the next), as in attn_fwd_ws_kernel -----------------
+__device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const PlanMaps& maps, uint32_t smem_q,
+                               uint32_t smem_kv, uint32_t bar0, uint32_t lead, WaitCtx& w) {
+  uint32_t slot = 0, empty_parity = 1;  // parity 1 passes on a fresh barrier
+  uint32_t q_empty_parity[kQTilesPerItem] = {1, 1};
+  uint32_t armed = 0, armed_parity = 0;  // for the early-exit path: "full" barriers armed, last parity of each
+  bool ok = true;
+  auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
+  const uint32_t q_bytes = uint32_t(p.tile_rows) * kHeadDim * 2;
+
+  auto push_pair = [&](const PlanPiece* v_pc, int v_tile, const PlanPiece* k_pc, int k_tile, int site) -> bool {
+    if (!w.wait_issue(bar(kPbPairEmpty + slot), empty_parity, site)) return false;
+    const uint32_t full_parity = empty_parity ^ 1u;
+    armed |= 1u << slot;
+    armed_parity = (armed_parity & ~(1u << slot)) | (full_parity << slot);
+    const uint32_t full = bar(kPbPairFull + slot);
+    const uint32_t dst = smem_kv + slot * kPairBytesP;
+    mbar_arrive_expect_tx_lead(lead, full, (v_pc != nullptr ? kTileBytes : 0) + (k_pc != nullptr ? kTileBytes : 0));
+    if (v_pc != nullptr) {
+      const CUtensorMap* tv = v_pc->source ? &maps.v_prefix : &maps.v;
+      const int row = v_pc->kv_row + v_tile * kBlockN, h = v_pc->kv_head;
+      tma_load_4d_lead(lead, dst, tv, 0, row, h, 0, full);
+      tma_load_4d_lead(lead, dst + kBoxBytes, tv, 64, row, h, 0, full);
+    }
+    if (k_pc != nullptr) {
+      const CUtensorMap* tk = k_pc->source ? &maps.k_prefix : &maps.k;
+      const int row = k_pc->kv_row + k_tile * kBlockN, h = k_pc->kv_head;
+      tma_load_4d_lead(lead, dst + kTileBytes, tk, 0, row, h, 0, full);
+      tma_load_4d_lead(lead, dst + kTileBytes + kBoxBytes, tk, 64, row, h, 0, full);
+    }
+    slot ^= 1u;
+    if (slot == 0) empty_parity ^= 1u;
+    return true;
+  };
+
+  PlanWalk walk(p, aux);
+  const PlanPiece* pc;
+  bool first = true;
+  while (ok && walk.take(pc)) {
+    const int T = piece_tiles(pc);
+    w.item = walk.i - 1;
+    w.tile = 0;
+    if (first) {
+      ok = push_pair(nullptr, 0, pc, 0, 110);  // the first K tile travels alone
+      first = false;
+      if (!ok) break;
+    }
+    for (int q = 0; ok && q < kQTilesPerItem; ++q) {
+      if (pc->tiles[q] == 0) continue;
+      ok = w.wait_issue(bar(kPbQEmpty + q), q_empty_parity[q], 100 + q);
+      if (!ok) break;
+      armed |= 1u << (kPairSlotsP + q);
+      armed_parity = (armed_parity & ~(1u << (kPairSlotsP + q))) | ((q_empty_parity[q] ^ 1u) << (kPairSlotsP + q));
+      q_empty_parity[q] ^= 1u;
+      // box of 64 columns x group heads x tile_tokens tokens: rows land as token * group + head
+      const uint32_t full = bar(kPbQFull + q), dst = smem_q + q * kTileBytes;
+      const int token = pc->token + q * p.tile_tokens;
+      mbar_arrive_expect_tx_lead(lead, full, q_bytes);
+      tma_load_4d_lead(lead, dst, &maps.q, 0, 0, pc->kv_head, token, full);
+      tma_load_4d_lead(lead, dst + kBoxBytes, &maps.q, 64, 0, pc->kv_head, token, full);
+    }
+    for (int i = 0; ok && i < T; ++i) {
+      w.tile = i;
+      if (i + 1 < T) {
+        ok = push_pair(pc, i, pc, i + 1, 111);
+      } else {
+        ok = push_pair(pc, i, walk.peek(), 0, 112);  // with the first K of the CTA's next piece, if any
+      }
+    }
+  }
+
+  if (!ok || w.aborted()) {
+    for (int s = 0; s < kPairSlotsP + kQTilesPerItem; ++s) {
+      if (!((armed >> s) & 1u)) continue;
+      const uint32_t b = (s < kPairSlotsP) ? bar(kPbPairFull + s) : bar(kPbQFull + (s - kPairSlotsP));
+      const uint64_t t0 = global_timer_ns();
+      while (!mbar_try_wait(b, (armed_parity >> s) & 1u, 1000)) {
+        if (global_timer_ns() - t0 > w.limit_ns) break;
+      }
+    }
+  }
+}
+
+// ---- V tails ------------------------------------------------------------------------------------------
+// Sees every pair (it takes part in handing pairs back, so it can never miss a phase). Where the V tile holds
+// the end of a piece's keys inside it, the rows behind are set to zero before the MMA warp may use the tile.
+__device__ void plan_tail_role(const PlanParams& p, const PlanAux* aux, uint8_t* kv, uint32_t bar0, int lane,
+                               WaitCtx& w) {
+  auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
+  uint32_t slot = 0, full_parity = 0;
+  auto next_pair = [&](int tail) -> bool {  // tail: keys in the V tile, 0 = all of them (or no V tile)
+    if (!w.wait_warp(bar(kPbPairFull + slot), full_parity, 600)) return false;
+    if (tail > 0) {
+      for (int box = 0; box < 2; ++box) {
+        uint4* row = reinterpret_cast<uint4*>(kv + slot * kPairBytesP + box * kBoxBytes + tail * 128);
+        const int words = (kBlockN - tail) * 8;
+        for (int j = lane; j < words; j += 32) row[j] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+    }
+    __syncwarp();
+    if (lane == 0) {
+      if (tail > 0) mbar_arrive(bar(kPbTailClean));
+      mbar_arrive(bar(kPbPairEmpty + slot));
+    }
+    slot ^= 1u;
+    if (slot == 0) full_parity ^= 1u;
+    return true;
+  };
+  PlanWalk walk(p, aux);
+  const PlanPiece* pc;
+  bool first = true;
+  while (walk.take(pc)) {
+    const int T = piece_tiles(pc);
+    w.item = walk.i - 1;
+    if (first && !next_pair(0)) return;
+    first = false;
+    for (int i = 0; i < T; ++i) {
+      w.tile = i;
+      if (!next_pair(i + 1 == T ? piece_tail(pc) : 0)) return;
+    }
+  }
+}
+
+// ---- MMA issuer ---------------------------------------------------------------------------------------
+__device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t smem_q, uint32_t smem_kv,
+                              uint32_t bar0, uint32_t tmem_base, uint32_t lead, WaitCtx& w) {
+  auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
+  uint32_t slot = 0, full_parity = 0, tail_parity = 0;
+  uint32_t q_full_parity[kQTilesPerItem] = {0, 0}, p_parity[kQTilesPerItem] = {0, 0};
+  uint32_t o_free_parity[kQTilesPerItem] = {1, 1};  // passes on the fresh barrier: both accumulators start out free
+  bool ok = true, k_ready = false;
+
+  PlanWalk walk(p, aux);
+  const PlanPiece* pc;
+  while (ok && walk.take(pc)) {
+    const int Tq[kQTilesPerItem] = {pc->tiles[0], pc->tiles[1]};
+    const int T = max(Tq[0], Tq[1]);
+    const bool tail = piece_tail(pc) > 0;
+    w.item = walk.i - 1;
+    w.tile = 0;
+    if (!k_ready) {
+      if (!(ok = w.wait_issue(bar(kPbPairFull + slot), full_parity, 200))) break;
+      slot ^= 1u;
+      if (slot == 0) full_parity ^= 1u;
+      k_ready = true;
+    }
+    {
+      const uint32_t k_smem = smem_kv + (slot ^ 1u) * kPairBytesP + kTileBytes;
+#pragma unroll
+      for (int q = 0; q < kQTilesPerItem; ++q) {
+        if (Tq[q] > 0) {
+          if (!(ok = w.wait_issue(bar(kPbQFull + q), q_full_parity[q], 201 + q))) break;
+          q_full_parity[q] ^= 1u;
+          tc_fence_after_sync();
+          issue_qk(lead, tmem_base + q * kBlockN, smem_q + q * kTileBytes, k_smem);
+          umma_commit_lead(lead, bar(kPbSFull + q));
+          if (Tq[q] == 1) umma_commit_lead(lead, bar(kPbQEmpty + q));
+        }
+      }
+    }
+    if (!ok) break;
+    // also covers the PV of the previous piece that read the V half of this pair
+    umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
+
+    for (int i = 0; ok && i < T; ++i) {
+      w.tile = i;
+      // V_i and K_{i+1} (or K_0 of this CTA's next piece) in one phase
+      if (!(ok = w.wait_issue(bar(kPbPairFull + slot), full_parity, 210))) break;
+      const uint32_t v_smem = smem_kv + slot * kPairBytesP;
+      const uint32_t k_smem = v_smem + kTileBytes;
+      const uint32_t pair_empty = bar(kPbPairEmpty + slot);
+      slot ^= 1u;
+      if (slot == 0) full_parity ^= 1u;
+      if (tail && i + 1 == T) {
+        if (!(ok = w.wait_issue(bar(kPbTailClean), tail_parity, 211))) break;
+        tail_parity ^= 1u;
+      }
+#pragma unroll
+      for (int q = 0; q < kQTilesPerItem; ++q) {
+        if (i < Tq[q]) {
+          const uint32_t s_tmem = tmem_base + q * kBlockN;
+          const uint32_t o_tmem = tmem_base + kQTilesPerItem * kBlockN + q * kHeadDim;
+          if (i == 0) {
+            // the previous piece's epilogue must have read O_q out before it is overwritten
+            if (!(ok = w.wait_issue(bar(kPbOFree + q), o_free_parity[q], 240 + q))) break;
+            o_free_parity[q] ^= 1u;
+          }
+          if (!(ok = w.wait_issue(bar(kPbPReady + q), p_parity[q], 220 + q))) break;
+          tc_fence_after_sync();
+          issue_pv(lead, o_tmem, s_tmem, v_smem, /*accumulate=*/i > 0);
+          p_parity[q] ^= 1u;
+          if (i + 1 < Tq[q]) {
+            issue_qk(lead, s_tmem, smem_q + q * kTileBytes, k_smem);
+            umma_commit_lead(lead, bar(kPbSFull + q));
+            if (i + 2 == Tq[q]) umma_commit_lead(lead, bar(kPbQEmpty + q));
+          } else {
+            umma_commit_lead(lead, bar(kPbPvDone + q));
+          }
+        }
+      }
+      if (ok && i + 1 < T) umma_commit_lead(lead, pair_empty);
+    }
+  }
+
+  if (!ok || w.aborted()) {
+    // Leaving early: make sure nothing this warp issued is still running before TMEM goes.
+    umma_commit_lead(lead, bar(kPbDrain));
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait(bar(kPbDrain), 0, 1000)) {
+      if (global_timer_ns() - t0 > w.limit_ns) break;
+    }
+  }
+}
+
+// ---- softmax: one row per thread -------------------------------------------------------------------------
+// As in attn_fwd_ws_kernel (speculative against the row's reference maximum, exact where the tile's sum says
+// that it has to move), plus rows that see no key of a tile, or of the whole piece: their m stays -inf, which
+// sends the row down the exact path, where it is subtracted as 0 so that every probability is 2^-inf = 0.
+__device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t bar0, uint32_t tmem_base, int q,
+                                  int warp_in_group, int lane, WaitCtx& w) {
+  auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
+  const float sum_limit = exp2f(B200ATTN_REBASE_LOG2);
+  const uint32_t lane_field = uint32_t(warp_in_group * 32) << 16;
+  const uint32_t s_tmem = tmem_base + q * kBlockN + lane_field;
+  const uint32_t p_tmem = s_tmem;  // bf16 P overwrites S columns 0..63
+  const uint32_t o_tmem = tmem_base + kQTilesPerItem * kBlockN + q * kHeadDim + lane_field;
+  const int r = warp_in_group * 32 + lane;
+  const int my_token = q * p.tile_tokens + min(r, p.tile_rows - 1) / p.group;  // of the block; idle rows go with the last
+  const float scale_log2 = p.scale_log2;
+  const f2 scale2 = f2_splat(scale_log2);
+  uint32_t s_parity = 0, fin_free_parity = 1;
+
+  PlanWalk walk(p, aux);
+  const PlanPiece* pc;
+  while (walk.take(pc)) {
+    const int T = pc->tiles[q];
+    if (T == 0) continue;
+    const int n_keys = pc->n_keys, diag = pc->diag;
+    // rows of this tile that exist; a warp without one only keeps the protocol going
+    const int rows = (min(pc->n_tokens - q * p.tile_tokens, p.tile_tokens)) * p.group;
+    const bool row_live = r < rows;
+    const bool warp_live = warp_in_group * 32 < rows;
+    const int tile_limit = min(n_keys - 1, diag + q * p.tile_tokens);  // last key that the tile's first row sees
+    const int row_limit = min(n_keys - 1, diag + my_token);            // last key that this row sees
+    w.item = walk.i - 1;
+    w.tile = 0;
+    if (!w.wait_warp(bar(kPbFinFree + q), fin_free_parity, 310 + q)) return;
+    fin_free_parity ^= 1u;
+    float m = kNegInf;  // reference maximum, log2 units
+    float l = 0.0f;     // running sum of 2^(s - m)
+    for (int i = 0; i < T; ++i) {
+      w.tile = i;
+      if (!w.wait_warp(bar(kPbSFull + q), s_parity, 300 + q)) return;
+      s_parity ^= 1u;
+      tc_fence_after_sync();
+      if (warp_live) {
+        uint32_t s[4][32];
+        tmem_ld32(s_tmem + 0, s[0]);
+        tmem_wait_ld();  // chunk 0 alone, so that its exponentials overlap the other three loads
+        tmem_ld32(s_tmem + 32, s[1]);
+        tmem_ld32(s_tmem + 64, s[2]);
+        tmem_ld32(s_tmem + 96, s[3]);
+        const bool tail = i * kBlockN + kBlockN - 1 > tile_limit;  // uniform across the warp
+        const int valid = row_limit - i * kBlockN + 1;             // keys of this tile that the row sees
+        if (tail || i == 0) tmem_wait_ld();
+        if (tail) mask_tail(s, valid);
+
+        uint32_t packed[4][16];
+        f2 sum_a = f2_splat(0.0f), sum_b = f2_splat(0.0f);
+        float tile_sum = 0.0f;
+        bool exact = (i == 0);
+        if (!exact) {
+          const f2 neg_m2 = f2_splat(-m);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            exp_chunk(s[c], scale2, neg_m2, packed[c], sum_a, sum_b);
+            if (c == 0) tmem_wait_ld();
+          }
+          tile_sum = f2_hsum(sum_a, sum_b);
+          // written so that a NaN sum also lands on the exact path
+          exact = __any_sync(0xffffffffu, row_live && !(tile_sum < sum_limit));
+        }
+        if (__builtin_expect(exact, 0)) {
+          if (i > 0) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, s[c]);
+            tmem_wait_ld();
+            if (tail) mask_tail(s, valid);
+          }
+          const float tile_max = row_max(s) * scale_log2;
+          const float m_new = fmaxf(m, tile_max);
+          if (i > 0) {
+            const float f = m_new == kNegInf ? 1.0f : ex2_approx(m - m_new);
+            l *= f;
+            if (__any_sync(0xffffffffu, f != 1.0f)) {
+#pragma unroll 1
+              for (int c = 0; c < kHeadDim / 16; ++c) {
+                uint32_t acc[16];
+                tmem_ld16(o_tmem + c * 16, acc);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[j] = __float_as_uint(__uint_as_float(acc[j]) * f);
+                tmem_st16(o_tmem + c * 16, acc);
+              }
+              tmem_wait_st();
+            }
+          }
+          m = m_new;
+          const f2 neg_m2 = f2_splat(m == kNegInf ? 0.0f : -m);
+          sum_a = f2_splat(0.0f);
+          sum_b = f2_splat(0.0f);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) exp_chunk(s[c], scale2, neg_m2, packed[c], sum_a, sum_b);
+          tile_sum = f2_hsum(sum_a, sum_b);
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_st16(p_tmem + c * 16, packed[c]);
+        tmem_wait_st();
+        l += tile_sum;
+      }
+      tc_fence_before_sync();
+      __syncwarp();
+      mbar_arrive_lead(lane == 0 ? 1u : 0u, bar(kPbPReady + q));
+    }
+    aux->row_max[q][r] = m;
+    aux->row_sum[q][r] = l;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kPbFin + q));
+  }
+}
+
+// ---- epilogue -----------------------------------------------------------------------------------------------
+__device__ void plan_epilogue_role(const PlanParams& p, const PlanAux* aux, uint32_t bar0, uint32_t tmem_base,
+                                   int warp_in_group, int lane, WaitCtx& w) {
+  auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
+  const uint32_t lane_field = uint32_t(warp_in_group * 32) << 16;
+  const int r = warp_in_group * 32 + lane;
+  const int token_in_tile = r / p.group, head_in_group = r - token_in_tile * p.group;
+  uint32_t fin_parity[kQTilesPerItem] = {0, 0};
+
+  PlanWalk walk(p, aux);
+  const PlanPiece* pc;
+  while (walk.take(pc)) {
+    w.item = walk.i - 1;
+    for (int q = 0; q < kQTilesPerItem; ++q) {
+      if (pc->tiles[q] == 0) continue;
+      w.tile = pc->tiles[q];
+      if (!w.wait_warp(bar(kPbFin + q), fin_parity[q], 410 + q)) return;
+      if (!w.wait_warp(bar(kPbPvDone + q), fin_parity[q], 420 + q)) return;
+      fin_parity[q] ^= 1u;
+      tc_fence_after_sync();
+      const float m = aux->row_max[q][r];
+      const float l = aux->row_sum[q][r];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kPbFinFree + q));
+      const int token = q * p.tile_tokens + token_in_tile;  // of the block
+      const bool live = r < p.tile_rows && token < pc->n_tokens;
+      const bool any_live = __any_sync(0xffffffffu, live);
+      const bool seen = l != 0.0f;  // false: the row saw no key (a NaN sum counts as seen)
+      const float weight = 1.0f / l;
+      const float lse = seen ? (m + log2f(l)) * kLn2 : kNegInf;
+      const int slot_row = pc->slot_row;
+      const int head = pc->kv_head * p.group + head_in_group;
+      const int64_t row = int64_t(pc->token) + token;
+      float* part = nullptr;
+      __nv_bfloat16* out = nullptr;
+      if (live) {
+        if (slot_row >= 0) {
+          const int64_t at = int64_t(slot_row) + token * p.group + head_in_group;
+          part = p.part_o + at * kHeadDim;
+          p.part_lse[at] = lse;
+        } else {
+          out = p.o + row * p.o_stride_t + int64_t(head) * p.o_stride_h;
+          if (p.lse != nullptr) p.lse[int64_t(head) * p.lse_stride_h + row] = lse;
+        }
+      }
+      const uint32_t o_row = tmem_base + kQTilesPerItem * kBlockN + q * kHeadDim + lane_field;
+      constexpr int kChunk = 16;
+      if (any_live) {
+#pragma unroll 1
+        for (int c = 0; c < kHeadDim / kChunk; ++c) {
+          uint32_t acc[kChunk];
+          tmem_ld16(o_row + c * kChunk, acc);
+          tmem_wait_ld();
+          if (!live) continue;
+          float v[kChunk];
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) v[j] = seen ? __uint_as_float(acc[j]) * weight : 0.0f;
+          if (slot_row >= 0) {
+            float4* dst = reinterpret_cast<float4*>(part + c * kChunk);
+#pragma unroll
+            for (int j = 0; j < kChunk / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(out + c * kChunk);
+#pragma unroll
+            for (int j = 0; j < kChunk / 8; ++j)
+              dst[j] = make_uint4(pack_bf16x2(v[8 * j + 0], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                                  pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+          }
+        }
+      }
+      // O_q has been read: the next piece's first PV may overwrite it
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kPbOFree + q));
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kPlanThreads, 1)
+attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  uint8_t* kv = smem + kQTilesPerItem * kTileBytes;
+  PlanAux* aux = reinterpret_cast<PlanAux*>(kv + kPairSlotsP * kPairBytesP);
+  const uint32_t smem_q = smem_u32(smem), smem_kv = smem_u32(kv);
+  const uint32_t bar0 = smem_u32(&aux->bar[0]);
+
+  WaitCtx w;
+  w.abort_addr = smem_u32(&aux->abort_flag);
+  w.status = p.status;
+  w.limit_ns = uint64_t(p.wait_limit_ms) * 1000000ull;
+  w.item = -1;
+  w.tile = -1;
+
+  const bool misaligned = (smem_q & 1023u) != 0;  // uniform across the CTA
+  const int piece0 = p.table[kPlanCtaAt + blockIdx.x], piece1 = p.table[kPlanCtaAt + blockIdx.x + 1];
+  if (piece0 >= piece1) return;  // uniform across the CTA: a table with fewer CTAs than the grid
+  if (threadIdx.x == 0) {
+    aux->abort_flag = 0;
+    aux->piece0 = piece0;
+    aux->piece1 = piece1;
+    if (misaligned) {
+      w.raise(kDevSmemMisaligned, 3, 0);
+    } else {
+      for (int q = 0; q < kQTilesPerItem; ++q) {
+        mbar_init(bar0 + 8u * (kPbQFull + q), 1);
+        mbar_init(bar0 + 8u * (kPbQEmpty + q), 1);
+        mbar_init(bar0 + 8u * (kPbSFull + q), 1);
+        mbar_init(bar0 + 8u * (kPbPReady + q), 4);
+        mbar_init(bar0 + 8u * (kPbPvDone + q), 1);
+        mbar_init(bar0 + 8u * (kPbFin + q), 4);
+        mbar_init(bar0 + 8u * (kPbFinFree + q), 4);
+        mbar_init(bar0 + 8u * (kPbOFree + q), 4);
+      }
+      for (int s = 0; s < kPairSlotsP; ++s) {
+        mbar_init(bar0 + 8u * (kPbPairFull + s), 1);
+        mbar_init(bar0 + 8u * (kPbPairEmpty + s), 2);
+      }
+      mbar_init(bar0 + 8u * kPbTailClean, 1);
+      mbar_init(bar0 + 8u * kPbDrain, 1);
+      mbar_init_fence();
+      fence_proxy_async_smem();
+    }
+  }
+  if (misaligned) return;
+  {
+    const int4* src = reinterpret_cast<const int4*>(p.table + kPlanPieceAt) + size_t(piece0) * 3;
+    int4* dst = reinterpret_cast<int4*>(aux->cache);
+    const int words = min(piece1 - piece0, kPieceCache) * 3;
+    for (int j = threadIdx.x; j < words; j += kPlanThreads) dst[j] = src[j];
+  }
+  if (warp == 12) {
+    tmem_alloc(smem_u32(&aux->tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = aux->tmem_base;
+
+  if (warp < 8) {
+    reg_grow<kPlanRegsSoftmax>();
+    plan_softmax_role(p, aux, bar0, tmem_base, warp >> 2, warp & 3, lane, w);
+  } else if (warp < 12) {
+    reg_shrink<kPlanRegsEpilogue>();
+    plan_epilogue_role(p, aux, bar0, tmem_base, warp & 3, lane, w);
+  } else {
+    reg_shrink<kPlanRegsOther>();
+    const uint32_t lead = (lane == 0) ? 1u : 0u;
+    if (warp == 12) {
+      plan_mma_role(p, aux, smem_q, smem_kv, bar0, tmem_base, lead, w);
+    } else if (warp == 13) {
+      plan_load_role(p, aux, maps, smem_q, smem_kv, bar0, lead, w);
+    } else if (warp == 14) {
+      plan_tail_role(p, aux, kv, bar0, lane, w);
+    }
+    __syncwarp();
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+// ---- join ---------------------------------------------------------------------------------------------------
+// A block per unit (at most 32 rows, or one token), a warp per row: the lanes find the row's total LSE over its
+// parts, then the warp adds the weighted partial rows, four in flight, lane l holding columns 4l .. 4l + 3.
+// Rows without a part get O = 0 and LSE = -inf. Reads 512 B per part and row: at 64 requests x 32 heads with
+// ten parts 10.5 MB, which the partials' stay in L2 makes a matter of latency.
+constexpr int kJoinWarps = 8;
+__global__ void __launch_bounds__(kJoinWarps * 32)
+attn_plan_join_kernel(const PlanParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int units = p.table[kPlanHdrUnits];
+  const PlanUnit* unit = reinterpret_cast<const PlanUnit*>(p.table + p.table[kPlanHdrUnitAt]);
+  const int32_t* part_list = p.table + p.table[kPlanHdrPartAt];
+  for (int u = blockIdx.x; u < units; u += gridDim.x) {
+    const PlanUnit un = unit[u];
+    const int32_t* parts = part_list + un.part0;
+    for (int r = warp; r < un.n_tokens * p.group; r += kJoinWarps) {
+      const int token = r / p.group;
+      const int head = un.kv_head * p.group + (r - token * p.group);
+      float top = kNegInf;
+      for (int k = lane; k < un.parts; k += 32) top = fmaxf(top, __ldcg(p.part_lse + parts[k] + r));
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const float base = top == kNegInf ? 0.0f : top;
+      float sum = 0.0f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k0 = 0; k0 < un.parts; k0 += 32) {
+        const int n = min(32, un.parts - k0);
+        float wgt = 0.0f;
+        int at = 0;
+        if (lane < n) {
+          at = parts[k0 + lane] + r;
+          wgt = expf(__ldcg(p.part_lse + at) - base);
+        }
+        sum += wgt;
+        for (int k = 0; k < n; k += 4) {
+          float4 a[4];
+          float ww[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int src = min(k + j, n - 1);
+            const int row = __shfl_sync(0xffffffffu, at, src);
+            ww[j] = __shfl_sync(0xffffffffu, wgt, src);
+            if (k + j >= n) ww[j] = 0.0f;
+            // a part without a visible key has weight 0 and a row of zeros
+            a[j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + int64_t(row) * kHeadDim) + lane);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (k + j < n) {
+              acc.x = fmaf(a[j].x, ww[j], acc.x);
+              acc.y = fmaf(a[j].y, ww[j], acc.y);
+              acc.z = fmaf(a[j].z, ww[j], acc.z);
+              acc.w = fmaf(a[j].w, ww[j], acc.w);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      const bool seen = sum != 0.0f;
+      const float inv = seen ? 1.0f / sum : 0.0f;
+      const int64_t row = int64_t(un.token) + token;
+      uint2 out;
+      out.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+      out.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>(p.o + row * p.o_stride_t + int64_t(head) * p.o_stride_h + lane * 4) = out;
+      if (p.lse != nullptr && lane == 0)
+        p.lse[int64_t(head) * p.lse_stride_h + row] = seen ? base + logf(sum) : kNegInf;
+    }
+  }
+}
+
+}  // namespace
+
+cudaError_t prepare_plan_kernels() {
+  constexpr int kPoolNeeded = 128 * (2 * kPlanRegsSoftmax + kPlanRegsEpilogue + kPlanRegsOther);
+  cudaFuncAttributes fa;
+  cudaError_t e = cudaFuncGetAttributes(&fa, attn_plan_kernel);
+  if (e != cudaSuccess) return e;
+  // a growing role would block in hardware if the launch did not reserve what the roles ask for
+  if (fa.numRegs * kPlanThreads < kPoolNeeded) return cudaErrorLaunchOutOfResources;
+  return cudaFuncSetAttribute(attn_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanSmemBytes);
+}
+
+cudaError_t launch_plan(const PlanMaps& maps, const PlanParams& p, int grid, cudaStream_t stream) {
+  attn_plan_kernel<<<grid, kPlanThreads, kPlanSmemBytes, stream>>>(maps, p);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_plan_join(const PlanParams& p, int grid, cudaStream_t stream) {
+  attn_plan_join_kernel<<<grid, kJoinWarps * 32, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace b200attn

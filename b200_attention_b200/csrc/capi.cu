@@ -4,6 +4,7 @@
 #include "../../include/b200_attention.h"
 #include "attn_kernels.cuh"
 #include "host_common.cuh"
+#include "plan_kernels.cuh"
 
 #include <atomic>
 #include <cmath>
@@ -93,6 +94,7 @@ void init_device(int device, DeviceState* st) {
     return;
   }
   e = prepare_kernels();
+  if (e == cudaSuccess) e = prepare_plan_kernels();
   if (e != cudaSuccess) {
     st->init_status = B200ATTN_ERR_CUDA;
     st->init_error = std::string("kernel attribute set-up: ") + cudaGetErrorString(e);
@@ -130,10 +132,20 @@ int get_device(int* device_out, DeviceState** st_out) {
 namespace b200attn {
 namespace host {
 
+int current_device(int* device, int* sm_count, int32_t** status) {
+  DeviceState* st = nullptr;
+  const int rc = get_device(device, &st);
+  if (rc != 0) return rc;
+  *sm_count = st->sm_count;
+  *status = st->status_dev;
+  return B200ATTN_OK;
+}
+
 // ---- tensor maps
 static bool same_key(const MapKey& a, const MapKey& o) {
   return a.ptr == o.ptr && a.sb == o.sb && a.sh == o.sh && a.sl == o.sl && a.batch == o.batch &&
-         a.heads == o.heads && a.len == o.len && a.device == o.device;
+         a.heads == o.heads && a.len == o.len && a.device == o.device && a.group == o.group &&
+         a.box_tokens == o.box_tokens;
 }
 
 struct MapCache {
@@ -163,11 +175,20 @@ int make_tensor_map(const MapKey& key, CUtensorMap* out) {
   auto legal = [](int64_t stride, int32_t extent) -> cuuint64_t {
     return cuuint64_t((extent == 1 && stride <= 0) ? kHeadDim : stride) * 2u;
   };
-  const cuuint64_t dims[4] = {cuuint64_t(kHeadDim), cuuint64_t(key.len), cuuint64_t(key.heads),
-                              cuuint64_t(key.batch)};
-  const cuuint64_t strides[3] = {legal(key.sl, key.len), legal(key.sh, key.heads),
-                                 legal(key.sb, key.batch)};
-  const cuuint32_t box[4] = {64, cuuint32_t(kBlockN), 1, 1};
+  cuuint64_t dims[4] = {cuuint64_t(kHeadDim), cuuint64_t(key.len), cuuint64_t(key.heads),
+                        cuuint64_t(key.batch)};
+  cuuint64_t strides[3] = {legal(key.sl, key.len), legal(key.sh, key.heads),
+                           legal(key.sb, key.batch)};
+  cuuint32_t box[4] = {64, cuuint32_t(kBlockN), 1, 1};
+  if (key.group > 0) {
+    dims[1] = cuuint64_t(key.group);
+    dims[3] = cuuint64_t(key.len);
+    strides[0] = legal(key.sh, key.group * key.heads);
+    strides[1] = strides[0] * cuuint64_t(key.group);
+    strides[2] = legal(key.sl, key.len);
+    box[1] = cuuint32_t(key.group);
+    box[3] = cuuint32_t(key.box_tokens);
+  }
   const cuuint32_t elem[4] = {1, 1, 1, 1};
   CUtensorMap map;
   const CUresult r = enc(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(key.ptr), dims,

@@ -27,10 +27,17 @@ struct MapKey {
   int64_t sb, sh, sl;  // strides in elements: batch, head, row
   int32_t batch, heads, len;
   int32_t device;
+  // Packed query view (group > 0): heads is the number of K/V heads, sh the stride of a query head, len the
+  // number of tokens; the map is (head_dim, head of the group, K/V head, token) with boxes of
+  // 64 x group x 1 x box_tokens.
+  int32_t group = 0, box_tokens = 0;
 };
 
 // Returns the cached map for `key`, encoding it on a miss (host-only work, no device memory).
 int make_tensor_map(const MapKey& key, CUtensorMap* out);
+
+// The current device, set up on first use: its index, SM count and the kernels' status record.
+int current_device(int* device, int* sm_count, int32_t** status);
 
 // Pointer / stride rules of one operand; reports through fail().
 int check_operand(const char* name, const b200attn_operand& t, int32_t batch, int32_t heads,

@@ -1,0 +1,324 @@
+// Host-side planner of the packed and shared-prefix attention calls: cuts the work into pieces,
+// deals them to CTAs and lists what has to be joined afterwards. No CUDA.
+//
+// An item is a block of 2 * floor(128 / group) tokens of one sequence and one K/V head with every
+// key it sees (for a shared prefix: a block of tokens of all sequences with the prefix). Items are
+// dealt to the CTA that is free first, longest first. Where that leaves CTAs idle at the end (few
+// or very unequal items) long items are cut into pieces of equal length first; the price of a cut is the
+// piece's own start and the join of the partial results. Which length is chosen is decided by
+// working out the finishing time for a handful of lengths.
+#include "plan.h"
+
+#include <algorithm>
+#include <queue>
+#include <utility>
+
+namespace b200attn {
+
+namespace {
+
+constexpr int kTile = 128;
+
+// Costs in thousandths of a K/V tile with two Q tiles on the tensor cores.
+constexpr int64_t kTilePair = 1000;    // two Q tiles against one K/V tile
+constexpr int64_t kTileSingle = 800;   // one Q tile: the same chain of steps without overlap
+constexpr int64_t kPieceStart = 1500;  // Q load, first scores, last PV, stores
+constexpr int64_t kJoin = 2500;        // the second kernel, once
+
+struct Item {
+  int32_t token, n_tokens, kv_row, n_keys, tiles0, tiles1, diag, kv_head, source;
+  int32_t sequence;  // -1: prefix
+  int32_t longest() const { return tiles1 > 0 ? tiles1 : tiles0; }
+};
+
+int64_t cost_of(int32_t tiles0, int32_t tiles1) {
+  return kPieceStart + (tiles1 > 0 ? int64_t(tiles1) * kTilePair : int64_t(tiles0) * kTileSingle);
+}
+
+// Piece `c` of an item cut every `len` tiles.
+PlanPiece cut_piece(const Item& it, int32_t from, int32_t len) {
+  PlanPiece p{};
+  p.token = it.token;
+  p.n_tokens = it.n_tokens;
+  p.kv_row = it.kv_row + from * kTile;
+  p.n_keys = int32_t(std::min<int64_t>(it.n_keys - int64_t(from) * kTile, int64_t(len) * kTile));
+  p.tiles[0] = std::max(0, std::min(it.tiles0 - from, len));
+  p.tiles[1] = std::max(0, std::min(it.tiles1 - from, len));
+  if (p.tiles[0] == 0) p.tiles[0] = 1;  // a fully masked tile: leaves an empty partial result
+  p.diag = it.diag == kPlanNoDiag ? kPlanNoDiag : it.diag - from * kTile;
+  p.kv_head = it.kv_head;
+  p.source = it.source;
+  p.slot_row = -1;
+  return p;
+}
+
+int32_t cuts_of(const Item& it, int32_t len) { return (it.longest() + len - 1) / len; }
+
+// Length of an item's pieces when none may exceed `len`: as equal as possible.
+int32_t even_len(const Item& it, int32_t len) {
+  const int32_t n = cuts_of(it, len);
+  return (it.longest() + n - 1) / n;
+}
+
+using Load = std::pair<int64_t, int32_t>;  // (busy until, CTA)
+using LoadQueue = std::priority_queue<Load, std::vector<Load>, std::greater<Load>>;
+
+LoadQueue empty_loads(int32_t ctas) {
+  std::vector<Load> v(static_cast<size_t>(ctas));
+  for (int32_t c = 0; c < ctas; ++c) v[size_t(c)] = {0, c};
+  return LoadQueue(std::greater<Load>(), std::move(v));
+}
+
+}  // namespace
+
+std::string plan_build(const PlanInput& in, Plan* plan) {
+  if (in.sequences < 1) return "there must be at least one sequence";
+  if (in.heads < 1 || in.heads_kv < 1 || in.heads % in.heads_kv != 0)
+    return "heads must be a positive multiple of heads_kv";
+  const int32_t group = in.heads / in.heads_kv;
+  if (group > 128) return "more than 128 query heads per K/V head";
+  if (in.sm_count < 1 || in.sm_count > kPlanMaxCtas) return "sm_count must be 1 .. 160";
+  if (in.len_prefix < 0 || in.len_prefix >= (1 << 30)) return "len_prefix must be 0 .. 2^30 - 1";
+
+  const int32_t tile_tokens = plan_tile_tokens(group);
+  const int32_t block = 2 * tile_tokens;
+  std::vector<int64_t> first_token(size_t(in.sequences) + 1, 0), first_key(size_t(in.sequences), 0);
+  int64_t at = 0;
+  plan->rows_kv = 0;
+  for (int32_t s = 0; s < in.sequences; ++s) {
+    const int64_t n = in.len_q[s], m = in.len_kv[s];
+    if (n < 0 || m < 0 || n >= (1 << 30) || m >= (1 << 30)) return "lengths must be 0 .. 2^30 - 1";
+    if (in.causal && in.len_prefix > 0 && m < n)
+      return "with a prefix and a causal mask a sequence needs at least as many keys of its own as queries";
+    first_token[size_t(s) + 1] = first_token[size_t(s)] + n;
+    const int64_t start = in.start_kv != nullptr ? in.start_kv[s] : at;
+    if (start < 0 || start + m >= (int64_t(1) << 31) - 256) return "K/V rows must be 0 .. 2^31 - 257";
+    first_key[size_t(s)] = start;
+    at += m;
+    if (m > 0) plan->rows_kv = std::max(plan->rows_kv, start + m);
+  }
+  plan->rows_q = first_token.back();
+  if (plan->rows_q >= (int64_t(1) << 31) - 256) return "too many query rows";
+
+  // ---- items
+  std::vector<Item> items;
+  int64_t kv_bytes = int64_t(in.len_prefix) * in.heads_kv * 512;
+  for (int32_t s = 0; s < in.sequences; ++s) {
+    const int32_t n = in.len_q[s], m = in.len_kv[s];
+    kv_bytes += int64_t(m) * in.heads_kv * 512;
+    if (m == 0) continue;
+    for (int32_t t = 0; t < n; t += block) {
+      Item it{};
+      it.sequence = s;
+      it.token = int32_t(first_token[size_t(s)]) + t;
+      it.n_tokens = std::min(block, n - t);
+      it.kv_row = int32_t(first_key[size_t(s)]);
+      it.n_keys = m;
+      it.diag = in.causal ? m - n + t : kPlanNoDiag;
+      int32_t tiles[2];
+      for (int32_t q = 0; q < 2; ++q) {
+        const int32_t here = std::min(tile_tokens, it.n_tokens - q * tile_tokens);  // tokens of Q tile q
+        if (here <= 0) {
+          tiles[q] = 0;
+          continue;
+        }
+        const int64_t keys = in.causal ? std::min<int64_t>(m, int64_t(it.diag) + q * tile_tokens + here) : m;
+        tiles[q] = keys <= 0 ? 0 : int32_t((keys + kTile - 1) / kTile);
+      }
+      if (tiles[0] == 0 && tiles[1] == 0) continue;  // no row of the block sees a key
+      it.tiles0 = std::max(1, tiles[0]);
+      it.tiles1 = tiles[1];
+      for (int32_t h = 0; h < in.heads_kv; ++h) {
+        it.kv_head = h;
+        items.push_back(it);
+      }
+    }
+  }
+  if (in.len_prefix > 0) {
+    const int32_t tiles = (in.len_prefix + kTile - 1) / kTile;
+    for (int64_t t = 0; t < plan->rows_q; t += block) {
+      Item it{};
+      it.sequence = -1;
+      it.token = int32_t(t);
+      it.n_tokens = int32_t(std::min<int64_t>(block, plan->rows_q - t));
+      it.kv_row = 0;
+      it.n_keys = in.len_prefix;
+      it.diag = kPlanNoDiag;
+      it.tiles0 = tiles;
+      it.tiles1 = it.n_tokens > tile_tokens ? tiles : 0;
+      it.source = 1;
+      for (int32_t h = 0; h < in.heads_kv; ++h) {
+        it.kv_head = h;
+        items.push_back(it);
+      }
+    }
+  }
+  const bool has_prefix = in.len_prefix > 0;
+
+  // ---- how long a piece may be
+  int64_t total_tiles = 0;
+  int32_t longest = 0;
+  for (const Item& it : items) {
+    total_tiles += it.longest();
+    longest = std::max(longest, it.longest());
+  }
+  int32_t best_len = std::max(longest, 1);
+  if (!items.empty()) {
+    std::vector<int32_t> lens{std::max(longest, 1)};
+    const int64_t even = (total_tiles + in.sm_count - 1) / in.sm_count;
+    for (const int64_t parts : {1, 2, 3, 4, 6, 8}) {
+      const int64_t len = std::max<int64_t>(2, (even + parts - 1) / parts);
+      if (len < longest && std::find(lens.begin(), lens.end(), int32_t(len)) == lens.end()) lens.push_back(int32_t(len));
+    }
+    int64_t best = -1;
+    std::vector<int64_t> costs;
+    for (const int32_t len : lens) {
+      costs.clear();
+      bool any_cut = has_prefix;
+      for (const Item& it : items) {
+        const int32_t n = cuts_of(it, len), l = even_len(it, len);
+        any_cut = any_cut || n > 1;
+        for (int32_t c = 0; c < n; ++c) {
+          const PlanPiece p = cut_piece(it, c * l, std::min(l, it.longest() - c * l));
+          costs.push_back(cost_of(p.tiles[0], p.tiles[1]));
+        }
+      }
+      std::sort(costs.begin(), costs.end(), std::greater<int64_t>());
+      LoadQueue q = empty_loads(in.sm_count);
+      int64_t end = 0;
+      for (const int64_t c : costs) {
+        const Load l = q.top();
+        q.pop();
+        q.push({l.first + c, l.second});
+        end = std::max(end, l.first + c);
+      }
+      end += any_cut ? kJoin : 0;
+      if (best < 0 || end < best) {
+        best = end;
+        best_len = len;
+      }
+    }
+  }
+
+  // ---- pieces, with the rows of their partial results
+  struct Piece {
+    PlanPiece p;
+    int64_t cost;
+    int32_t head_group;
+  };
+  // K/V of sixteen heads at a time where all of it would not stay in L2 (see CausalWalk's groups)
+  const bool by_groups = kv_bytes > (int64_t(64) << 20);
+  std::vector<Piece> pieces;
+  std::vector<int32_t> item_piece0(items.size() + 1, 0);
+  int64_t slots = 0;
+  for (size_t i = 0; i < items.size(); ++i) {
+    const Item& it = items[i];
+    item_piece0[i] = int32_t(pieces.size());
+    const int32_t n = cuts_of(it, best_len), l = even_len(it, best_len);
+    for (int32_t c = 0; c < n; ++c) {
+      Piece p{};
+      p.p = cut_piece(it, c * l, std::min(l, it.longest() - c * l));
+      if (n > 1 || has_prefix) {
+        p.p.slot_row = int32_t(slots);
+        slots += int64_t(it.n_tokens) * group;
+        if (slots >= (int64_t(1) << 31) - 512) return "too many partial rows";
+      }
+      p.cost = cost_of(p.p.tiles[0], p.p.tiles[1]);
+      p.head_group = by_groups ? it.kv_head / 16 : 0;
+      pieces.push_back(p);
+    }
+  }
+  item_piece0[items.size()] = int32_t(pieces.size());
+  if (pieces.size() >= (size_t(1) << 24)) return "too many pieces";
+  plan->slot_rows = slots;
+  plan->pieces = int32_t(pieces.size());
+
+  // ---- join units
+  std::vector<PlanUnit> units;
+  std::vector<int32_t> parts;
+  const int32_t unit_tokens = std::max(1, kPlanJoinRows / group);
+  const int32_t heads_kv = in.heads_kv;
+  // items of a (sequence, block) are heads_kv consecutive entries, in the order they were made
+  size_t next_own = 0;
+  size_t prefix_at = items.size();
+  if (has_prefix) prefix_at = items.size() - size_t((plan->rows_q + block - 1) / block) * size_t(heads_kv);
+  for (int32_t s = 0; s < in.sequences; ++s) {
+    const int32_t n = in.len_q[s];
+    for (int32_t t = 0; t < n; t += block) {
+      const int32_t token = int32_t(first_token[size_t(s)]) + t;
+      const int32_t here = std::min(block, n - t);
+      const bool own = next_own < prefix_at && items[next_own].sequence == s && items[next_own].token == token;
+      for (int32_t h = 0; h < heads_kv; ++h) {
+        const size_t own_item = next_own + size_t(h);
+        if (own && !has_prefix && item_piece0[own_item + 1] - item_piece0[own_item] == 1) continue;  // wrote o itself
+        for (int32_t i = 0; i < here;) {
+          int32_t count = std::min(unit_tokens, here - i);
+          PlanUnit u{};
+          u.token = token + i;
+          u.part0 = int32_t(parts.size());
+          u.kv_head = h;
+          if (has_prefix) {
+            const int32_t b = u.token / block;  // a unit stays inside one block of the prefix's items
+            count = std::min(count, (b + 1) * block - u.token);
+            const size_t item = prefix_at + size_t(b) * size_t(heads_kv) + size_t(h);
+            for (int32_t p = item_piece0[item]; p < item_piece0[item + 1]; ++p)
+              parts.push_back(pieces[size_t(p)].p.slot_row + (u.token - b * block) * group);
+          }
+          if (own)
+            for (int32_t p = item_piece0[own_item]; p < item_piece0[own_item + 1]; ++p)
+              parts.push_back(pieces[size_t(p)].p.slot_row + i * group);
+          u.n_tokens = count;
+          u.parts = int32_t(parts.size()) - u.part0;
+          units.push_back(u);
+          i += count;
+        }
+      }
+      if (own) next_own += size_t(heads_kv);
+    }
+  }
+  if (units.size() >= (size_t(1) << 28) || parts.size() >= (size_t(1) << 28)) return "too many rows to join";
+  plan->units = int32_t(units.size());
+
+  // ---- dealing: longest first, each to the CTA that is free first
+  std::vector<int32_t> order(pieces.size());
+  for (size_t i = 0; i < order.size(); ++i) order[i] = int32_t(i);
+  std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) {
+    const Piece &x = pieces[size_t(a)], &y = pieces[size_t(b)];
+    if (x.head_group != y.head_group) return x.head_group < y.head_group;
+    return x.cost > y.cost;
+  });
+  std::vector<std::vector<int32_t>> dealt(size_t(in.sm_count));
+  LoadQueue q = empty_loads(in.sm_count);
+  for (const int32_t i : order) {
+    const Load l = q.top();
+    q.pop();
+    dealt[size_t(l.second)].push_back(i);
+    q.push({l.first + pieces[size_t(i)].cost, l.second});
+  }
+  plan->grid = 0;
+  for (int32_t c = 0; c < in.sm_count; ++c)
+    if (!dealt[size_t(c)].empty()) plan->grid = c + 1;
+
+  // ---- table
+  const size_t unit_at = size_t(kPlanPieceAt) + pieces.size() * (sizeof(PlanPiece) / 4);
+  const size_t part_at = unit_at + units.size() * (sizeof(PlanUnit) / 4);
+  plan->table.assign((part_at + parts.size() + 3) / 4 * 4, 0);
+  int32_t* t = plan->table.data();
+  t[kPlanHdrMagic] = kPlanMagic;
+  t[kPlanHdrPieces] = plan->pieces;
+  t[kPlanHdrUnits] = plan->units;
+  t[kPlanHdrUnitAt] = int32_t(unit_at);
+  t[kPlanHdrPartAt] = int32_t(part_at);
+  PlanPiece* out = reinterpret_cast<PlanPiece*>(t + kPlanPieceAt);
+  int32_t k = 0;
+  for (int32_t c = 0; c <= kPlanMaxCtas; ++c) {
+    t[kPlanCtaAt + c] = k;
+    if (c < in.sm_count)
+      for (const int32_t i : dealt[size_t(c)]) out[k++] = pieces[size_t(i)].p;
+  }
+  std::copy(units.begin(), units.end(), reinterpret_cast<PlanUnit*>(t + unit_at));
+  std::copy(parts.begin(), parts.end(), t + part_at);
+  return "";
+}
+
+}  // namespace b200attn

@@ -1,0 +1,33 @@
+// Internal interface between the C-ABI layer and the planned-attention and rotation kernels.
+#pragma once
+
+#include "attn_kernels.cuh"
+#include "plan.h"
+
+namespace b200attn {
+
+// q: (head_dim, head of the group, K/V head, token); the others: (head_dim, row, K/V head, 1)
+struct PlanMaps {
+  CUtensorMap q, k, v, k_prefix, v_prefix;
+};
+
+struct PlanParams {
+  const int32_t* table;
+  __nv_bfloat16* o;
+  float* lse;  // [heads][lse_stride_h], or null
+  int64_t o_stride_t, o_stride_h, lse_stride_h;
+  float* part_o;    // [slot rows][128] fp32, normalised
+  float* part_lse;  // [slot rows], natural log, -inf where no key was visible
+  int32_t group;        // query heads per K/V head
+  int32_t tile_tokens;  // floor(128 / group)
+  int32_t tile_rows;    // tile_tokens * group
+  float scale_log2;
+  int32_t* status;
+  uint32_t wait_limit_ms;
+};
+
+cudaError_t prepare_plan_kernels();
+cudaError_t launch_plan(const PlanMaps& maps, const PlanParams& p, int grid, cudaStream_t stream);
+cudaError_t launch_plan_join(const PlanParams& p, int grid, cudaStream_t stream);
+
+}  // namespace b200attn

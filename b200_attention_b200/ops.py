@@ -14,6 +14,8 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native as N
+from .packed import AttentionPlan, attention_packed, attention_shared_prefix  # noqa: F401
+from .rotary import qk_norm_rope  # noqa: F401
 
 HEAD_DIM = 128
 

@@ -1,0 +1,278 @@
+"""Attention over packed sequences of different lengths, and over requests that share a prefix.
+
+    plan = AttentionPlan(lens_q, lens_kv, heads=32, heads_kv=8, causal=True)   # once per batch
+    o = attention_packed(q, k, v, plan)                                        # every layer
+
+    plan = AttentionPlan(lens_q, lens_kv, heads=32, heads_kv=8, len_prefix=len(k_prefix))
+    o = attention_shared_prefix(q, k_prefix, v_prefix, k, v, plan)
+
+Sequences lie back to back: q and o are [rows, heads, 128], k and v [rows, heads_kv, 128]; k and v may also be a
+cache in which every sequence has rows of its own (`starts_kv`). A plan is made on the host from the lengths and
+says which CTA works on what (see b200attn_plan_create); it depends on nothing else and serves every call with
+those lengths. A whole prompt, a later chunk of one and a single new token are the same call with other lengths.
+
+The reference project has no counterpart: its kernels take one rectangular problem.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional, Sequence
+
+import torch
+
+from . import _native as N
+
+HEAD_DIM = 128
+
+
+def _int_list(name: str, values) -> list:
+    if isinstance(values, torch.Tensor):
+        if values.is_cuda:
+            raise RuntimeError(f"{name} must be host integers: a plan is made on the host")
+        if values.dim() != 1 or values.dtype.is_floating_point or values.dtype in (torch.bool, torch.complex64):
+            raise TypeError(f"{name} must be a 1-D tensor of integers")
+        return values.tolist()
+    out = []
+    for v in values:
+        i = v.__index__() if hasattr(v, "__index__") and not isinstance(v, bool) else None
+        if i is None:
+            raise TypeError(f"{name} must hold integers, got {v!r}")
+        out.append(i)
+    return out
+
+
+class Schedule:
+    """A plan's host side: sizes (`info`) and table (int32, host), from host arithmetic only."""
+
+    def __init__(self, lens_q, lens_kv, *, heads: int, heads_kv: Optional[int] = None, causal: bool = True,
+                 starts_kv=None, len_prefix: int = 0, sm_count: int = 0):
+        lq, lk = _int_list("lens_q", lens_q), _int_list("lens_kv", lens_kv)
+        if len(lq) != len(lk):
+            raise ValueError(f"lens_q holds {len(lq)} lengths, lens_kv {len(lk)}")
+        st = None if starts_kv is None else _int_list("starts_kv", starts_kv)
+        if st is not None and len(st) != len(lk):
+            raise ValueError(f"starts_kv holds {len(st)} rows, lens_kv {len(lk)} lengths")
+        for name, vals, top in (("lens_q", lq, 2**30), ("lens_kv", lk, 2**30), ("starts_kv", st or (), 2**31)):
+            if any(not 0 <= x < top for x in vals):
+                raise ValueError(f"{name} must be 0 .. {top - 1}")
+        for name, x in (("heads", heads), ("heads_kv", heads_kv), ("len_prefix", len_prefix)):
+            if x is not None and not -2**31 <= x < 2**31:
+                raise ValueError(f"{name} is out of range")
+        self.sequences, self.heads, self.heads_kv = len(lq), int(heads), int(heads if heads_kv is None else heads_kv)
+        self.causal, self.len_prefix = bool(causal), int(len_prefix)
+        n = max(1, len(lq))
+        d = N.PlanDesc()
+        d.struct_bytes = C.sizeof(N.PlanDesc)
+        d.sequences, d.heads, d.heads_kv = len(lq), self.heads, self.heads_kv
+        d.causal, d.len_prefix, d.sm_count = int(self.causal), self.len_prefix, int(sm_count)
+        d.len_q, d.len_kv = (C.c_int32 * n)(*lq), (C.c_int32 * n)(*lk)
+        if st is not None:
+            d.start_kv = (C.c_int64 * n)(*st)
+        self.info = N.PlanInfo()
+        self.info.struct_bytes = C.sizeof(N.PlanInfo)
+        handle = C.c_void_p()
+        lib = N.lib()
+        N.check(lib.b200attn_plan_create(C.byref(d), C.byref(self.info), C.byref(handle)))
+        try:
+            self.table = torch.empty(self.info.table_bytes // 4, dtype=torch.int32)
+            N.check(lib.b200attn_plan_table(handle, self.table.data_ptr(), self.info.table_bytes))
+        finally:
+            lib.b200attn_plan_destroy(handle)
+
+
+class AttentionPlan:
+    """Which CTA works on what, for sequences of the given lengths.
+
+    lens_q, lens_kv: tokens and keys of each sequence (host integers; 0 allowed). heads_kv: K/V heads (default: as
+    many as heads; query head h reads K/V head h // (heads // heads_kv)). causal: token i of n sees key j of m iff
+    j <= i + (m - n), so a sequence's last token sees all of its keys. starts_kv: first row of each sequence in
+    k and v; default: back to back. len_prefix: rows of a shared prefix that every token sees in front of its own
+    keys (attention_shared_prefix). device: where the calls will run (default: the current CUDA device).
+
+    `update` puts other lengths in place. Calls captured into a CUDA graph read the plan's table when the graph is
+    replayed, so an updated plan changes what the replay does; `update` refuses lengths that a captured call has no
+    room for. A plan may be used on any stream of its device, also by overlapping calls; only `update` must not overlap
+    calls that use it on other streams than the current one.
+    """
+
+    def __init__(self, lens_q, lens_kv, *, heads: int, heads_kv: Optional[int] = None, causal: bool = True,
+                 starts_kv=None, len_prefix: int = 0, device=None):
+        s = Schedule(lens_q, lens_kv, heads=heads, heads_kv=heads_kv, causal=causal, starts_kv=starts_kv,
+                     len_prefix=len_prefix)
+        device = torch.device("cuda" if device is None else device)
+        if device.type != "cuda":
+            raise RuntimeError("a plan needs a CUDA device (this library has no CPU path)")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        if torch.cuda.get_device_properties(device).multi_processor_count != 148:
+            s = Schedule(lens_q, lens_kv, heads=heads, heads_kv=heads_kv, causal=causal, starts_kv=starts_kv,
+                         len_prefix=len_prefix,
+                         sm_count=min(160, torch.cuda.get_device_properties(device).multi_processor_count))
+        self.device = device
+        self.heads, self.heads_kv, self.causal, self.len_prefix = s.heads, s.heads_kv, s.causal, s.len_prefix
+        self._sm_count = min(160, torch.cuda.get_device_properties(device).multi_processor_count)
+        # room for the schedules of other lengths: twice this one's, and a little for small ones
+        self._room_units = 2 * s.info.units + 1024
+        self._room_slots = 2 * s.info.slot_rows + 4096
+        self._captured = None  # (rows of q, rows of k) that every captured call has at least
+        self._table = torch.zeros(2 * s.table.numel() + 16384, dtype=torch.int32, device=device)
+        self._put(s)
+
+    def _put(self, s: Schedule) -> None:
+        with torch.cuda.device(self.device):
+            # The copy is complete when this returns, so calls on any stream find the table. Host memory here is
+            # pageable: nothing of it is read after that either.
+            self._table[: s.table.numel()].copy_(s.table)
+            torch.cuda.current_stream().synchronize()
+        i = s.info
+        self.rows_q, self.rows_kv = i.rows_q, i.rows_kv
+        self._grid, self._units, self._slots = i.grid, i.units, i.slot_rows
+
+    def update(self, lens_q, lens_kv, *, starts_kv=None) -> None:
+        """Other lengths, same heads, mask and prefix. Takes effect for calls made after it and for replays started
+        after it, in the order of the current stream; waits for that stream."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a plan cannot be updated while the current stream is being captured")
+        s = Schedule(lens_q, lens_kv, heads=self.heads, heads_kv=self.heads_kv, causal=self.causal,
+                     starts_kv=starts_kv, len_prefix=self.len_prefix, sm_count=self._sm_count)
+        fits = (s.table.numel() <= self._table.numel() and s.info.units <= self._room_units
+                and s.info.slot_rows <= self._room_slots)
+        if self._captured is not None:
+            rows_q, rows_kv = self._captured
+            if not fits or s.info.rows_q > rows_q or s.info.rows_kv > rows_kv:
+                raise RuntimeError("these lengths do not fit the calls captured with this plan; make a new plan and "
+                                   "capture again")
+        elif not fits:
+            self._room_units, self._room_slots = 2 * s.info.units + 1024, 2 * s.info.slot_rows + 4096
+            self._table = torch.zeros(2 * s.table.numel() + 16384, dtype=torch.int32, device=self.device)
+        self._put(s)
+
+
+def _check_rows(name: str, t, heads: int, device) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor (this library has no CPU path)")
+    if t.dtype != torch.bfloat16:
+        raise RuntimeError(f"{name} must be bfloat16, got {t.dtype}")
+    if t.dim() != 3 or t.size(2) != HEAD_DIM:
+        raise RuntimeError(f"{name} must be [rows, heads, {HEAD_DIM}], got {tuple(t.shape)}")
+    if t.stride(2) != 1:
+        raise RuntimeError(f"{name}: the head_dim axis must be contiguous")
+    if t.size(1) != heads:
+        raise RuntimeError(f"{name} has {t.size(1)} heads, the plan {heads}")
+    if t.device != device:
+        raise RuntimeError(f"{name} is on {t.device}, the plan on {device}")
+
+
+def _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream):
+    if not isinstance(plan, AttentionPlan):
+        raise TypeError("plan must be an AttentionPlan")
+    given = [("q", q, plan.heads), ("k", k, plan.heads_kv), ("v", v, plan.heads_kv)]
+    if k_prefix is not None:
+        given += [("k_prefix", k_prefix, plan.heads_kv), ("v_prefix", v_prefix, plan.heads_kv)]
+    for name, t, heads in given:
+        _check_rows(name, t, heads, plan.device)
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} requires grad: this library computes forward passes only")
+    if k.size(0) != v.size(0):
+        raise RuntimeError(f"k has {k.size(0)} rows, v {v.size(0)}")
+    if q.size(0) < plan.rows_q:
+        raise RuntimeError(f"q has {q.size(0)} rows, the plan covers {plan.rows_q}")
+    if k.size(0) < plan.rows_kv:
+        raise RuntimeError(f"k and v have {k.size(0)} rows, the plan reads up to row {plan.rows_kv}")
+    for name, t in (("q", q), ("k", k)):
+        if t.size(0) >= 2**31 - 256:
+            raise RuntimeError(f"{name} has too many rows")
+    if out is not None:
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
+            raise RuntimeError("out must match q in shape, dtype and device with a dense head_dim axis")
+    if torch.cuda.current_device() != plan.device.index:
+        with torch.cuda.device(plan.device):
+            return _launch(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream)
+    return _launch(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream)
+
+
+def _launch(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream):
+    current = torch.cuda.current_stream()
+    if stream is not None and stream != current:
+        with torch.cuda.stream(stream):
+            return _launch(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
+    rows = q.size(0)
+    lse = torch.empty((plan.heads, rows), dtype=torch.float32, device=q.device) if return_lse else None
+    if out is None:
+        out = torch.empty((rows, plan.heads, HEAD_DIM), dtype=q.dtype, device=q.device)
+        if rows > plan.rows_q:
+            out[plan.rows_q:].zero_()
+    if lse is not None and rows > plan.rows_q:
+        lse[:, plan.rows_q:].fill_(-torch.inf)
+    if torch.cuda.is_current_stream_capturing():
+        # a replay may find the table of other lengths: launch for all that may be in it
+        grid, units, slots = plan._sm_count, plan._room_units, plan._room_slots
+        if k.size(0) == 0 and plan.len_prefix == 0:
+            grid = 0
+        held = plan._captured or (rows, k.size(0))
+        plan._captured = (min(held[0], rows), min(held[1], k.size(0)))
+    else:
+        grid, units, slots = plan._grid, plan._units, plan._slots
+    if rows > 0 and (grid > 0 or units > 0):
+        a = N.PlannedArgs()
+        a.struct_bytes = C.sizeof(N.PlannedArgs)
+        a.heads, a.heads_kv, a.head_dim = plan.heads, plan.heads_kv, HEAD_DIM
+        a.rows_q, a.rows_kv, a.len_prefix = rows, k.size(0), plan.len_prefix
+        a.grid, a.join_units = grid, units
+        for name, t in (("q", q), ("k", k), ("v", v), ("k_prefix", k_prefix), ("v_prefix", v_prefix), ("o", out)):
+            if t is not None:
+                setattr(a, name, N.Operand(t.data_ptr(), 0, t.stride(1), t.stride(0)))
+        if lse is not None:
+            a.lse, a.lse_stride_head = lse.data_ptr(), rows
+        a.softmax_scale = float(softmax_scale)
+        a.table = plan._table.data_ptr()
+        # From the caching allocator at every call: in stream order, and private to a graph that is being captured.
+        workspace = torch.empty(slots * (HEAD_DIM + 1), dtype=torch.float32, device=q.device) if slots else None
+        if workspace is not None:
+            a.workspace, a.slot_rows = workspace.data_ptr(), slots
+        a.stream = current.cuda_stream
+        N.check(N.lib().b200attn_forward_planned(C.byref(a)))
+    return (out, lse) if return_lse else out
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttentionPlan, *,
+                     softmax_scale: float = 0.0, return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                     stream: Optional[torch.cuda.Stream] = None):
+    """O = softmax(Q K^T * scale) V for every sequence of the plan, on the current CUDA stream.
+
+    q: [rows, heads, 128] bf16, the sequences' tokens back to back; k, v: [rows, heads_kv, 128]. Any strides that are
+    multiples of 8 elements (at least 128), head_dim dense. Returns O like q and, if asked, LSE [heads, rows] fp32
+    (natural log). A token that sees no key gets O = 0 and LSE = -inf. Rows of q behind the plan's last sequence are
+    not read; their rows of a given `out` keep what they hold, in an O made here they are 0 (LSE: -inf). Rows of
+    k and v outside the plan's sequences have no influence, whatever they hold. `out` must not overlap k or v.
+    Forward only. softmax_scale <= 0: 1 / sqrt(128).
+    """
+    if isinstance(plan, AttentionPlan) and plan.len_prefix:
+        raise RuntimeError("this plan has a prefix: use attention_shared_prefix")
+    return _run(q, k, v, None, None, plan, softmax_scale, return_lse, out, stream)
+
+
+def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor,
+                            v: torch.Tensor, plan: AttentionPlan, *, softmax_scale: float = 0.0,
+                            return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                            stream: Optional[torch.cuda.Stream] = None):
+    """As attention_packed, with every token also seeing all of a prefix [len_prefix, heads_kv, 128] in front of its
+    sequence's own keys. The prefix is read for blocks of tokens of all sequences together, not once per sequence.
+    k_prefix, v_prefix: at least the plan's len_prefix rows (the first ones are used).
+    """
+    if not isinstance(plan, AttentionPlan):
+        raise TypeError("plan must be an AttentionPlan")
+    if not plan.len_prefix:
+        raise RuntimeError("this plan has no prefix: use attention_packed")
+    for name, t in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.dim() < 1 or t.size(0) < plan.len_prefix:
+            raise RuntimeError(f"{name} has fewer than the plan's {plan.len_prefix} rows")
+    return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream)
+
+
+__all__ = ["AttentionPlan", "Schedule", "attention_packed", "attention_shared_prefix"]

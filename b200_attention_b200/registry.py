@@ -75,7 +75,7 @@ def sha256_file(path: Path) -> str:
 def source_closure_sha256(spec: KernelSpec) -> str:
     """Fingerprint of the kernel source and every header it includes (cf. registry.py:230-255)."""
     h = hashlib.sha256()
-    names = ["csrc/attn_fwd_sm100.cu", "csrc/capi.cu", "csrc/noalloc.cu", "csrc/attn_kernels.cuh",
+    names = ["csrc/attn_fwd_sm100.cu", "csrc/capi.cu", "csrc/noalloc.cu", "csrc/attn_device_sm100.cuh", "csrc/attn_kernels.cuh",
              "csrc/ptx_sm100.cuh", "csrc/host_common.cuh", "../include/b200_attention.h"]
     for name in names:
         p = (PKG / name).resolve()

@@ -187,6 +187,101 @@ B200ATTN_API int b200attn_copy_async(void* dst_local, const void* src, uint64_t 
 #define B200ATTN_NOALLOC_MAX_ROWS 16384
 B200ATTN_API int b200attn_forward_kv_split_noalloc(const b200attn_forward_args* args, int32_t kv_splits);
 
+/* ---- Planned attention: packed sequences, shared prefixes (no counterpart in the reference) ----------
+ *
+ * Sequences of different lengths lie back to back in q and o ([rows, heads, 128]) and, back to back or at
+ * rows of the caller's choice, in k and v ([rows, heads_kv, 128]). Query head h reads K/V head
+ * h / (heads / heads_kv). A plan, made on the host from the lengths alone, says which CTA does what; it
+ * serves every call with those lengths (every layer of a step). With len_prefix > 0 every query also sees
+ * the first len_prefix rows of a second pair (k_prefix, v_prefix), in front of its sequence's own keys.
+ *   causal != 0: token i of n sees key j of m of its own keys iff j <= i + (m - n). A row that sees no key gets
+ *                O = 0 and LSE = -inf. With a prefix, m >= n is required. */
+typedef struct b200attn_plan_desc {
+  uint32_t struct_bytes; /* sizeof(b200attn_plan_desc), checked */
+  int32_t sequences;     /* >= 1 */
+  int32_t heads, heads_kv; /* heads a multiple of heads_kv, at most 128 query heads per K/V head */
+  int32_t causal;
+  int32_t len_prefix; /* 0: none */
+  int32_t sm_count;   /* 0: 148 */
+  int32_t reserved;   /* 0 */
+  const int32_t* len_q;    /* [sequences], host memory, 0 allowed */
+  const int32_t* len_kv;   /* [sequences], host memory, 0 allowed */
+  const int64_t* start_kv; /* [sequences] first row of each in k and v, host memory; NULL: back to back */
+} b200attn_plan_desc;
+
+typedef struct b200attn_plan_info {
+  uint32_t struct_bytes; /* sizeof(b200attn_plan_info), checked */
+  int32_t grid;          /* CTAs with work */
+  int32_t pieces;        /* pieces of work */
+  int32_t units;         /* groups of rows that are joined from partial results */
+  int64_t rows_q;        /* rows of q and o that the plan covers */
+  int64_t rows_kv;       /* rows of k and v that it may read */
+  int64_t slot_rows;     /* rows of partial results */
+  uint64_t table_bytes;
+  uint64_t workspace_bytes; /* of b200attn_planned_args.workspace: slot_rows * 516 */
+} b200attn_plan_info;
+
+/* Host arithmetic only, needs no device. On success *plan is a handle for the two calls below. */
+B200ATTN_API int b200attn_plan_create(const b200attn_plan_desc* desc, b200attn_plan_info* info, void** plan);
+/* Copies the plan's table (info.table_bytes) to host memory; the caller brings it to the device. */
+B200ATTN_API int b200attn_plan_table(const void* plan, void* table, uint64_t bytes);
+B200ATTN_API int b200attn_plan_destroy(void* plan);
+
+typedef struct b200attn_planned_args {
+  uint32_t struct_bytes; /* sizeof(b200attn_planned_args), checked */
+  int32_t heads, heads_kv, head_dim; /* as planned; head_dim 128 */
+  int32_t rows_q;     /* rows of q and o, at least info.rows_q; the rest are neither read nor written */
+  int32_t rows_kv;    /* rows of k and v, at least info.rows_kv */
+  int32_t len_prefix; /* as planned */
+  int32_t grid;       /* info.grid, or more where the table may be replaced before a replay; <= 160 */
+  int32_t join_units; /* info.units, or more in the same way; 0: nothing is joined */
+  int32_t reserved;   /* 0 */
+  b200attn_operand q, k, v, k_prefix, v_prefix; /* bf16; stride_batch is not used */
+  b200attn_operand o;                           /* bf16, written */
+  float* lse;              /* [heads, >= rows_q] fp32, natural log; may be NULL */
+  int64_t lse_stride_head; /* elements between heads of lse */
+  float softmax_scale;     /* <= 0 selects 1/sqrt(head_dim) */
+  int32_t reserved2;       /* 0 */
+  const void* table;       /* device memory, 16-byte aligned */
+  void* workspace;         /* device memory, 16-byte aligned, slot_rows * 516 bytes, any contents; calls
+                            * that may overlap need workspaces of their own */
+  int64_t slot_rows;       /* rows the workspace has room for, at least info.slot_rows */
+  void* stream;
+} b200attn_planned_args;
+
+/* Asynchronous on args->stream: one kernel, and a second one where rows are joined. The table is taken as it is:
+ * it must come from b200attn_plan_table for the sizes given here. */
+B200ATTN_API int b200attn_forward_planned(const b200attn_planned_args* args);
+
+/* ---- Norm and rotation of queries and keys (no counterpart in the reference) -----------------------------
+ *
+ * For each token and head, 128 values: y = x * rsqrt(mean(x^2) + eps) * weight (where a weight is given), then
+ * pair j of y is turned by position[axis(j)] * inv_freq[j]: (a, b) -> (a cos - b sin, b cos + a sin). Pairs are
+ * (j, j + 64), or (2j, 2j + 1) if interleaved. The first section[0] pairs take their position from axis 0, the
+ * next section[1] from axis 1, and so on; pairs behind the last section are not turned. q_out and k_out may be
+ * q and k themselves; otherwise they must not overlap them. */
+typedef struct b200attn_qk_norm_rope_args {
+  uint32_t struct_bytes; /* sizeof(b200attn_qk_norm_rope_args), checked */
+  int32_t batch, tokens, heads_q, heads_k, head_dim; /* heads_k may be 0 (k, k_out unused); head_dim 128 */
+  b200attn_operand q, k, q_out, k_out;               /* bf16; strides of batch, head, token */
+  const void* q_weight; /* [128] or NULL: no norm */
+  const void* k_weight;
+  int32_t weight_type;   /* 0 bf16, 1 fp32 */
+  int32_t position_type; /* 0 int32, 1 int64, 2 fp32 */
+  const void* positions; /* device memory, element (axis, batch, token) by the strides below */
+  int64_t position_stride_axis, position_stride_batch, position_stride_token;
+  const float* inv_freq; /* [sum of sections] */
+  int32_t axes;          /* 1 .. 4 */
+  int32_t section[4];    /* pairs of each axis, sum 1 .. 64 */
+  float eps;
+  int32_t interleaved;
+  int32_t reserved; /* 0 */
+  void* stream;
+} b200attn_qk_norm_rope_args;
+
+/* Asynchronous on args->stream: one kernel. */
+B200ATTN_API int b200attn_qk_norm_rope(const b200attn_qk_norm_rope_args* args);
+
 B200ATTN_API const char* b200attn_status_string(int status);
 /* Message of the last failing call on this thread ("" if none). */
 B200ATTN_API const char* b200attn_last_error(void);
