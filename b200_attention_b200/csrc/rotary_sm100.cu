@@ -4,13 +4,21 @@
 //   pair j of y:  (a, b) -> (a cos t - b sin t, b cos t + a sin t),  t = position[axis(j)] * inv_freq[j]
 //   pairs are (j, j + 64), or (2j, 2j + 1) when interleaved; pairs behind the last section stay as they are
 //
-// Bound by memory: 512 bytes per head and token for about 10 operations per value. A warp takes one token, half a
-// warp one head: a lane holds eight values of a head, which are four whole pairs in either pairing, so the only
-// exchange is the sum of squares over 16 lanes. The angles depend on the token and the pair alone: a lane works
-// its four out once and uses them for every head that the warp visits.
+// Bound by memory: 512 bytes per head and token, and not far from being bound by instructions: about 10 operations per
+// value. A warp takes one token, a quarter of a warp one head: a lane holds values 8l .. 8l + 7 and 64 + 8l .. 64 + 8l + 7,
+// which are eight whole pairs in either pairing, so the only exchange is the sum of squares over eight lanes. The
+// angles depend on the token and the pair alone: each lane works out two, through shared memory they reach the lanes
+// that need them, and they serve every head that the warp visits. The rotation is linear, so the norm's weight goes
+// into the cosines and sines once per token and only the row's scale is left to apply per head; arithmetic is on
+// packed pairs of 32-bit values.
+// Measured at 16384 tokens, 32 + 8 heads: half a warp per head with every lane working out its own four angles ran
+// 47.6 M warp instructions and was bound by them (71 us, 4.7 TB/s); this form takes 61.5 us, 5.5 TB/s, 85 % of what a
+// plain copy reaches. Blocks of 4 warps with 2 heads ahead against 8 warps: 63.4 and 65.1 us; 1 head ahead and more
+// warps per SM: 67.5 us.
 // Statistics and rotation are in 32 bits and rounded to bf16 once. Angles are reduced to a fraction of a turn in
 // 64 bits first: at position 10^6 a 32-bit product is already off by 0.03 radians.
 
+#include "ptx_sm100.cuh"
 #include "rotary_kernels.cuh"
 
 #include <cuda_bf16.h>
@@ -19,12 +27,23 @@ namespace b200attn {
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kHeadsPerStep = 4;  // heads that a half warp has in flight
+using ptx::f2;
+using ptx::f2_fma;
+using ptx::f2_make;
+using ptx::f2_split;
+using ptx::f2_splat;
+using ptx::pack_bf16x2;
 
-struct alignas(8) Half4 {
-  __nv_bfloat162 lo, hi;
-};
+constexpr int kWarps = 4;
+constexpr int kBlocksPerSm = 6;  // 85 registers: 24 warps with two heads each on their way hold 48 KB of loads per SM
+constexpr int kPairs = 64;
+constexpr int kDepth = 2;  // heads of a quarter warp that are on their way while one is worked on
+
+__device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
 
 __device__ __forceinline__ double position_of(const RotaryParams& p, int axis, int64_t b, int64_t t) {
   const int64_t at = axis * p.pos_stride_axis + b * p.pos_stride_batch + t * p.pos_stride_token;
@@ -33,116 +52,164 @@ __device__ __forceinline__ double position_of(const RotaryParams& p, int axis, i
   return double(static_cast<const float*>(p.positions)[at]);
 }
 
-__device__ __forceinline__ void unpack4(uint2 raw, float (&v)[4]) {
-  v[0] = __uint_as_float(raw.x << 16);
-  v[1] = __uint_as_float(raw.x & 0xffff0000u);
-  v[2] = __uint_as_float(raw.y << 16);
-  v[3] = __uint_as_float(raw.y & 0xffff0000u);
-}
+// Nothing reads the result again before much else has gone through the L2: marked as such (3 % at 16384 tokens).
+__device__ __forceinline__ void store16(char* p, uint4 v) { __stcs(reinterpret_cast<uint4*>(p), v); }
 
-__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
-  union {
-    Half4 h;
-    uint2 u;
-  } r;
-  r.h.lo = __floats2bfloat162_rn(a, b);
-  r.h.hi = __floats2bfloat162_rn(c, d);
-  return r.u;
+// Two bf16 of a word, in order and exchanged.
+__device__ __forceinline__ f2 unpack2(uint32_t w) {
+  return f2_make(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ f2 unpack2_swapped(uint32_t w) {
+  return f2_make(__uint_as_float(w & 0xffff0000u), __uint_as_float(w << 16));
+}
+__device__ __forceinline__ uint32_t pack2(f2 v) {
+  float lo, hi;
+  f2_split(v, lo, hi);
+  return pack_bf16x2(lo, hi);
 }
 
 __device__ __forceinline__ float weight_of(const void* w, int is_fp32, int i) {
+  if (w == nullptr) return 1.0f;
   return is_fp32 ? static_cast<const float*>(w)[i] : __bfloat162float(static_cast<const __nv_bfloat16*>(w)[i]);
 }
 
-// kInterleaved: values 8l .. 8l + 7 of a head in lane l of a half warp; otherwise 4l .. 4l + 3 and 64 + 4l .. + 3.
-// Either way a[i], b[i] are the two values of pair 4l + i.
-template <bool kInterleaved>
-__global__ void __launch_bounds__(kWarps * 32) qk_norm_rope_kernel(const RotaryParams p) {
-  const int lane = threadIdx.x & 31, l = lane & 15, half = lane >> 4;
-  const int64_t unit = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t row = unit / p.chunks;
-  if (row >= int64_t(p.batch) * p.tokens) return;
-  const int chunk = int(unit - row * p.chunks);
-  const int64_t b = row / p.tokens, t = row - b * p.tokens;
-
-  float cosv[4], sinv[4];
+// Heads h0, h0 + 4, .. < end of one operand for the calling quarter warp (h0 already counts the quarter).
+// `turn` holds (cos, sin) of the token's 64 pairs and is ready once `angles` has been called.
+template <bool kInterleaved, class Angles>
+__device__ __forceinline__ void rotate_heads(const RotaryOperand& x, const RotaryParams& p, int64_t b, int64_t t, int h0,
+                                             int end, int l, const float2* turn, const float* w, Angles angles) {
+  const char* src = reinterpret_cast<const char*>(x.in + b * x.in_stride_b + t * x.in_stride_t + h0 * x.in_stride_h + 8 * l);
+  char* dst = reinterpret_cast<char*>(x.out + b * x.out_stride_b + t * x.out_stride_t + h0 * x.out_stride_h + 8 * l);
+  const int64_t src_step = x.in_stride_h * 8, dst_step = x.out_stride_h * 8;  // four heads, in bytes
+  uint4 raw[kDepth][2];
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) {
+    raw[d][0] = raw[d][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (h0 + 4 * d < end) {
+      raw[d][0] = *reinterpret_cast<const uint4*>(src + d * src_step);
+      raw[d][1] = *reinterpret_cast<const uint4*>(src + d * src_step + 128);
+    }
+  }
+  angles();
+  // Packed coefficients. Pairs (j, j + 64): values (e0 e1)(e2 e3).. of the lower half with (f0 f1).. of the upper half,
+  //   e' = e (w_e cos) + f (-w_f sin), f' = f (w_f cos) + e (w_e sin).
+  // Pairs (2j, 2j + 1): the word (e f) itself, (e' f') = (e f)(w_e cos, w_f cos) + (f e)(-w_f sin, w_e sin).
+  f2 cos_lo[4], cos_hi[4], sin_lo[4], sin_hi[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int j = 4 * l + i;
-    cosv[i] = 1.0f;
-    sinv[i] = 0.0f;
-    if (j < p.pairs) {
-      int axis = 0;
-#pragma unroll
-      for (int a = 0; a < kRotaryMaxAxes - 1; ++a) axis += (j >= p.section_end[a]) ? 1 : 0;
-      const double turns = position_of(p, axis, b, t) * (double(p.inv_freq[j]) * 0.15915494309189535);
-      sincospif(2.0f * float(turns - rint(turns)), &sinv[i], &cosv[i]);
+    const float2 w0 = *reinterpret_cast<const float2*>(w + 8 * l + 2 * i);
+    const float2 w1 = *reinterpret_cast<const float2*>(w + 64 + 8 * l + 2 * i);
+    if (kInterleaved) {
+      const float2 c0 = turn[4 * l + i], c1 = turn[32 + 4 * l + i];
+      cos_lo[i] = f2_make(w0.x * c0.x, w0.y * c0.x);
+      sin_lo[i] = f2_make(-w0.y * c0.y, w0.x * c0.y);
+      cos_hi[i] = f2_make(w1.x * c1.x, w1.y * c1.x);
+      sin_hi[i] = f2_make(-w1.y * c1.y, w1.x * c1.y);
+    } else {
+      const float4 cs = *reinterpret_cast<const float4*>(turn + 8 * l + 2 * i);
+      cos_lo[i] = f2_make(w0.x * cs.x, w0.y * cs.z);
+      cos_hi[i] = f2_make(w1.x * cs.x, w1.y * cs.z);
+      sin_lo[i] = f2_make(-w1.x * cs.y, -w1.y * cs.w);
+      sin_hi[i] = f2_make(w0.x * cs.y, w0.y * cs.w);
     }
   }
-
-  const int heads = p.heads_q + p.heads_k;
-  const int first = chunk * p.chunk_heads, end = min(heads, first + p.chunk_heads);
-  for (int h0 = first; h0 < end; h0 += 2 * kHeadsPerStep) {
-    uint2 raw[kHeadsPerStep][2];
+  const bool norm = x.weight != nullptr;
+  for (int h = h0; __any_sync(0xffffffffu, h < end); h += 4 * kDepth) {
 #pragma unroll
-    for (int s = 0; s < kHeadsPerStep; ++s) {
-      const int h = h0 + 2 * s + half;
-      if (h < end) {
-        const bool is_k = h >= p.heads_q;
-        const RotaryOperand& x = is_k ? p.k : p.q;
-        const __nv_bfloat16* src = x.in + b * x.in_stride_b + int64_t(is_k ? h - p.heads_q : h) * x.in_stride_h + t * x.in_stride_t;
-        if (kInterleaved) {
-          const uint4 r = *reinterpret_cast<const uint4*>(src + 8 * l);
-          raw[s][0] = make_uint2(r.x, r.y);
-          raw[s][1] = make_uint2(r.z, r.w);
-        } else {
-          raw[s][0] = *reinterpret_cast<const uint2*>(src + 4 * l);
-          raw[s][1] = *reinterpret_cast<const uint2*>(src + 64 + 4 * l);
-        }
-      } else {
-        raw[s][0] = raw[s][1] = make_uint2(0u, 0u);
+    for (int d = 0; d < kDepth; ++d) {
+      const uint32_t lo[4] = {raw[d][0].x, raw[d][0].y, raw[d][0].z, raw[d][0].w};
+      const uint32_t hi[4] = {raw[d][1].x, raw[d][1].y, raw[d][1].z, raw[d][1].w};
+      const bool live = h + 4 * d < end;
+      if (h + 4 * (d + kDepth) < end) {
+        raw[d][0] = *reinterpret_cast<const uint4*>(src + (d + kDepth) * src_step);
+        raw[d][1] = *reinterpret_cast<const uint4*>(src + (d + kDepth) * src_step + 128);
       }
-    }
-#pragma unroll
-    for (int s = 0; s < kHeadsPerStep; ++s) {
-      const int h = h0 + 2 * s + half;
-      const bool is_k = h >= p.heads_q;
-      const RotaryOperand& x = is_k ? p.k : p.q;
-      float v[2][4];
-      unpack4(raw[s][0], v[0]);
-      unpack4(raw[s][1], v[1]);
-      float sq = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sq = fmaf(v[0][i], v[0][i], fmaf(v[1][i], v[1][i], sq));
-#pragma unroll
-      for (int d = 8; d > 0; d >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, d);
-      if (h >= end) continue;
-      if (x.weight != nullptr) {
-        const float scale = rsqrtf(sq * (1.0f / 128.0f) + p.eps);
+      f2 scale = f2_splat(1.0f);
+      if (norm) {
+        f2 sq0 = f2_splat(0.0f), sq1 = f2_splat(0.0f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          v[0][i] *= scale * weight_of(x.weight, p.weight_fp32, kInterleaved ? 8 * l + i : 4 * l + i);
-          v[1][i] *= scale * weight_of(x.weight, p.weight_fp32, kInterleaved ? 8 * l + 4 + i : 64 + 4 * l + i);
+          const f2 e = unpack2(lo[i]), f = unpack2(hi[i]);
+          sq0 = f2_fma(e, e, sq0);
+          sq1 = f2_fma(f, f, sq1);
         }
+        float a, c;
+        f2_split(ptx::f2_add(sq0, sq1), a, c);
+        float sq = a + c;
+        sq += __shfl_xor_sync(0xffffffffu, sq, 4);
+        sq += __shfl_xor_sync(0xffffffffu, sq, 2);
+        sq += __shfl_xor_sync(0xffffffffu, sq, 1);
+        scale = f2_splat(rsqrtf(fmaf(sq, 1.0f / 128.0f, p.eps)));
       }
-      float a[4], c[4];
+      uint32_t out_lo[4], out_hi[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float e = kInterleaved ? v[i >> 1][2 * (i & 1)] : v[0][i];
-        const float f = kInterleaved ? v[i >> 1][2 * (i & 1) + 1] : v[1][i];
-        a[i] = e * cosv[i] - f * sinv[i];
-        c[i] = f * cosv[i] + e * sinv[i];
+        const f2 e = unpack2(lo[i]), f = unpack2(hi[i]);
+        f2 a, c;
+        if (kInterleaved) {
+          a = f2_fma(e, cos_lo[i], f2_mul(unpack2_swapped(lo[i]), sin_lo[i]));
+          c = f2_fma(f, cos_hi[i], f2_mul(unpack2_swapped(hi[i]), sin_hi[i]));
+        } else {
+          a = f2_fma(e, cos_lo[i], f2_mul(f, sin_lo[i]));
+          c = f2_fma(f, cos_hi[i], f2_mul(e, sin_hi[i]));
+        }
+        if (norm) {
+          a = f2_mul(a, scale);
+          c = f2_mul(c, scale);
+        }
+        out_lo[i] = pack2(a);
+        out_hi[i] = pack2(c);
       }
-      __nv_bfloat16* dst = x.out + b * x.out_stride_b + int64_t(is_k ? h - p.heads_q : h) * x.out_stride_h + t * x.out_stride_t;
-      if (kInterleaved) {
-        const uint2 lo = pack4(a[0], c[0], a[1], c[1]), hi = pack4(a[2], c[2], a[3], c[3]);
-        *reinterpret_cast<uint4*>(dst + 8 * l) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      } else {
-        *reinterpret_cast<uint2*>(dst + 4 * l) = pack4(a[0], a[1], a[2], a[3]);
-        *reinterpret_cast<uint2*>(dst + 64 + 4 * l) = pack4(c[0], c[1], c[2], c[3]);
+      if (live) {
+        store16(dst + d * dst_step, make_uint4(out_lo[0], out_lo[1], out_lo[2], out_lo[3]));
+        store16(dst + d * dst_step + 128, make_uint4(out_hi[0], out_hi[1], out_hi[2], out_hi[3]));
       }
     }
+    src += kDepth * src_step;
+    dst += kDepth * dst_step;
   }
+}
+
+template <bool kInterleaved>
+__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_norm_rope_kernel(const RotaryParams p) {
+  __shared__ alignas(16) float2 turns_of[kWarps][kPairs];
+  __shared__ alignas(16) float weights[2][128];  // 1 where there is none
+  for (int i = threadIdx.x; i < 256; i += kWarps * 32)
+    weights[i >> 7][i & 127] = weight_of((i >> 7) ? p.k.weight : p.q.weight, p.weight_fp32, i & 127);
+  __syncthreads();
+  const int lane = threadIdx.x & 31, l = lane & 7, quarter = lane >> 3;
+  const int64_t unit = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+  const int64_t row = unit / p.chunks;
+  if (row >= int64_t(p.batch) * p.tokens) return;  // whole warps
+  const int chunk = int(unit - row * p.chunks);
+  const int64_t b = row / p.tokens, t = row - b * p.tokens;
+  float2* turn = turns_of[threadIdx.x >> 5];
+
+  bool have = false;
+  auto angles = [&]() {
+    if (have) return;
+    have = true;
+#pragma unroll
+    for (int i = 0; i < kPairs / 32; ++i) {
+      const int j = lane + 32 * i;
+      float2 cs = make_float2(1.0f, 0.0f);
+      if (j < p.pairs) {
+        int axis = 0;
+#pragma unroll
+        for (int a = 0; a < kRotaryMaxAxes - 1; ++a) axis += (j >= p.section_end[a]) ? 1 : 0;
+        const double turns = position_of(p, axis, b, t) * (double(p.inv_freq[j]) * 0.15915494309189535);
+        sincospif(2.0f * float(turns - rint(turns)), &cs.y, &cs.x);
+      }
+      turn[j] = cs;
+    }
+    __syncwarp();
+  };
+  // a warp's heads: some of q's, or of k's, or the last of q's and the first of k's
+  const int first = chunk * p.chunk_heads, end = min(p.heads_q + p.heads_k, first + p.chunk_heads);
+  if (first < p.heads_q)
+    rotate_heads<kInterleaved>(p.q, p, b, t, first + quarter, min(end, p.heads_q), l, turn, weights[0], angles);
+  if (end > p.heads_q)
+    rotate_heads<kInterleaved>(p.k, p, b, t, max(first, p.heads_q) - p.heads_q + quarter, end - p.heads_q, l, turn, weights[1], angles);
 }
 
 }  // namespace
@@ -154,10 +221,10 @@ cudaError_t launch_qk_norm_rope(RotaryParams p, bool interleaved, int sm_count, 
   const int64_t wanted = int64_t(sm_count) * 32;
   int chunks = 1;
   if (rows < wanted) {
-    const int64_t most = (heads + 1) / 2;
+    const int64_t most = (heads + 3) / 4;
     chunks = int((wanted + rows - 1) / rows < most ? (wanted + rows - 1) / rows : most);
   }
-  p.chunk_heads = ((heads + chunks - 1) / chunks + 1) / 2 * 2;
+  p.chunk_heads = ((heads + chunks - 1) / chunks + 3) / 4 * 4;
   p.chunks = (heads + p.chunk_heads - 1) / p.chunk_heads;
   const int64_t blocks = (rows * p.chunks + kWarps - 1) / kWarps;
   if (interleaved)

@@ -17,13 +17,11 @@ The reference project has no counterpart: its kernels take one rectangular probl
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence
+from typing import Optional
 
 import torch
 
 from . import _native as N
-
-HEAD_DIM = 128
 
 
 def _int_list(name: str, values) -> list:
@@ -127,7 +125,15 @@ class AttentionPlan:
             torch.cuda.current_stream().synchronize()
         i = s.info
         self.rows_q, self.rows_kv = i.rows_q, i.rows_kv
-        self._grid, self._units, self._slots = i.grid, i.units, i.slot_rows
+        self._now = [self.heads, self.heads_kv, i.rows_q, i.rows_kv, self.len_prefix, i.grid, i.units, i.slot_rows]
+
+    def _for_capture(self, k) -> list:
+        grid = self._sm_count if k.size(0) or self.len_prefix else 0
+        return self._now[:5] + [grid, self._room_units, self._room_slots]
+
+    def _hold(self, rows_q: int, rows_kv: int) -> None:
+        held = self._captured or (rows_q, rows_kv)
+        self._captured = (min(held[0], rows_q), min(held[1], rows_kv))
 
     def update(self, lens_q, lens_kv, *, starts_kv=None) -> None:
         """Other lengths, same heads, mask and prefix. Takes effect for calls made after it and for replays started
@@ -149,93 +155,66 @@ class AttentionPlan:
         self._put(s)
 
 
-def _check_rows(name: str, t, heads: int, device) -> None:
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor (this library has no CPU path)")
-    if t.dtype != torch.bfloat16:
-        raise RuntimeError(f"{name} must be bfloat16, got {t.dtype}")
-    if t.dim() != 3 or t.size(2) != HEAD_DIM:
-        raise RuntimeError(f"{name} must be [rows, heads, {HEAD_DIM}], got {tuple(t.shape)}")
-    if t.stride(2) != 1:
-        raise RuntimeError(f"{name}: the head_dim axis must be contiguous")
-    if t.size(1) != heads:
-        raise RuntimeError(f"{name} has {t.size(1)} heads, the plan {heads}")
-    if t.device != device:
-        raise RuntimeError(f"{name} is on {t.device}, the plan on {device}")
-
-
 def _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream):
     if not isinstance(plan, AttentionPlan):
         raise TypeError("plan must be an AttentionPlan")
-    given = [("q", q, plan.heads), ("k", k, plan.heads_kv), ("v", v, plan.heads_kv)]
-    if k_prefix is not None:
-        given += [("k_prefix", k_prefix, plan.heads_kv), ("v_prefix", v_prefix, plan.heads_kv)]
-    for name, t, heads in given:
-        _check_rows(name, t, heads, plan.device)
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError(f"{name} requires grad: this library computes forward passes only")
-    if k.size(0) != v.size(0):
-        raise RuntimeError(f"k has {k.size(0)} rows, v {v.size(0)}")
-    if q.size(0) < plan.rows_q:
-        raise RuntimeError(f"q has {q.size(0)} rows, the plan covers {plan.rows_q}")
-    if k.size(0) < plan.rows_kv:
-        raise RuntimeError(f"k and v have {k.size(0)} rows, the plan reads up to row {plan.rows_kv}")
-    for name, t in (("q", q), ("k", k)):
-        if t.size(0) >= 2**31 - 256:
-            raise RuntimeError(f"{name} has too many rows")
-    if out is not None:
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1:
-            raise RuntimeError("out must match q in shape, dtype and device with a dense head_dim axis")
-    if torch.cuda.current_device() != plan.device.index:
-        with torch.cuda.device(plan.device):
-            return _launch(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream)
-    return _launch(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream)
-
-
-def _launch(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream):
-    current = torch.cuda.current_stream()
-    if stream is not None and stream != current:
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+    if stream is not None and stream != torch.cuda.current_stream(plan.device):
         with torch.cuda.stream(stream):
-            return _launch(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
-    rows = q.size(0)
-    lse = torch.empty((plan.heads, rows), dtype=torch.float32, device=q.device) if return_lse else None
-    if out is None:
-        out = torch.empty((rows, plan.heads, HEAD_DIM), dtype=q.dtype, device=q.device)
-        if rows > plan.rows_q:
-            out[plan.rows_q:].zero_()
-    if lse is not None and rows > plan.rows_q:
-        lse[:, plan.rows_q:].fill_(-torch.inf)
-    if torch.cuda.is_current_stream_capturing():
-        # a replay may find the table of other lengths: launch for all that may be in it
-        grid, units, slots = plan._sm_count, plan._room_units, plan._room_slots
-        if k.size(0) == 0 and plan.len_prefix == 0:
-            grid = 0
-        held = plan._captured or (rows, k.size(0))
-        plan._captured = (min(held[0], rows), min(held[1], k.size(0)))
-    else:
-        grid, units, slots = plan._grid, plan._units, plan._slots
-    if rows > 0 and (grid > 0 or units > 0):
-        a = N.PlannedArgs()
-        a.struct_bytes = C.sizeof(N.PlannedArgs)
-        a.heads, a.heads_kv, a.head_dim = plan.heads, plan.heads_kv, HEAD_DIM
-        a.rows_q, a.rows_kv, a.len_prefix = rows, k.size(0), plan.len_prefix
-        a.grid, a.join_units = grid, units
-        for name, t in (("q", q), ("k", k), ("v", v), ("k_prefix", k_prefix), ("v_prefix", v_prefix), ("o", out)):
-            if t is not None:
-                setattr(a, name, N.Operand(t.data_ptr(), 0, t.stride(1), t.stride(0)))
-        if lse is not None:
-            a.lse, a.lse_stride_head = lse.data_ptr(), rows
-        a.softmax_scale = float(softmax_scale)
-        a.table = plan._table.data_ptr()
-        # From the caching allocator at every call: in stream order, and private to a graph that is being captured.
-        workspace = torch.empty(slots * (HEAD_DIM + 1), dtype=torch.float32, device=q.device) if slots else None
-        if workspace is not None:
-            a.workspace, a.slot_rows = workspace.data_ptr(), slots
-        a.stream = current.cuda_stream
-        N.check(N.lib().b200attn_forward_planned(C.byref(a)))
-    return (out, lse) if return_lse else out
+            return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
+    # a replay may find the table of other lengths: a captured call launches for all that may be in it
+    capturing = torch.cuda.is_current_stream_capturing()
+    o, lse = N.torch_ops().attention_planned(q, k, v, k_prefix, v_prefix, plan._table,
+                                             plan._for_capture(k) if capturing else plan._now, softmax_scale,
+                                             return_lse, out)
+    if capturing:
+        plan._hold(q.size(0), k.size(0))
+    return (o, lse) if return_lse else o
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttentionPlan, *,
+                     softmax_scale: float = 0.0, return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                     stream: Optional[torch.cuda.Stream] = None):
+    """O = softmax(Q K^T * scale) V for every sequence of the plan, on the current CUDA stream.
+
+    q: [rows, heads, 128] bf16, the sequences' tokens back to back; k, v: [rows, heads_kv, 128]. Any strides that are
+    multiples of 8 elements (at least 128), head_dim dense. Returns O like q and, if asked, LSE [heads, rows] fp32
+    (natural log). A token that sees no key gets O = 0 and LSE = -inf. Rows of q behind the plan's last sequence are
+    not read; their rows of a given `out` keep what they hold, in an O made here they are 0 (LSE: -inf). Rows of
+    k and v outside the plan's sequences have no influence, whatever they hold. `out` must not overlap k or v.
+    Forward only. softmax_scale <= 0: 1 / sqrt(128).
+    """
+    if isinstance(plan, AttentionPlan) and plan.len_prefix:
+        raise RuntimeError("this plan has a prefix: use attention_shared_prefix")
+    return _run(q, k, v, None, None, plan, softmax_scale, return_lse, out, stream)
+
+
+def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor,
+                            v: torch.Tensor, plan: AttentionPlan, *, softmax_scale: float = 0.0,
+                            return_lse: bool = False, out: Optional[torch.Tensor] = None,
+                            stream: Optional[torch.cuda.Stream] = None):
+    """As attention_packed, with every token also seeing all of a prefix [len_prefix, heads_kv, 128] in front of its
+    sequence's own keys. The prefix is read for blocks of tokens of all sequences together, not once per sequence.
+    k_prefix, v_prefix: at least the plan's len_prefix rows (the first ones are used).
+    """
+    if not isinstance(plan, AttentionPlan):
+        raise TypeError("plan must be an AttentionPlan")
+    if not plan.len_prefix:
+        raise RuntimeError("this plan has no prefix: use attention_packed")
+    for name, t in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+    return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
+    # a replay may find the table of other lengths: a captured call launches for all that may be in it
+    capturing = torch.cuda.is_current_stream_capturing()
+    o, lse = N.torch_ops().attention_planned(q, k, v, k_prefix, v_prefix, plan._table,
+                                             plan._for_capture(k) if capturing else plan._now, softmax_scale,
+                                             return_lse, out)
+    if capturing:
+        plan._hold(q.size(0), k.size(0))
+    return (o, lse) if return_lse else o
 
 
 def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttentionPlan, *,

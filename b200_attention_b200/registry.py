@@ -102,18 +102,6 @@ class _KernelModule:
         self._ns.device_check()
 
 
-_loaded = False
-
-
 def load_kernel(spec: KernelSpec) -> _KernelModule:
     """Loads libb200attn.so and the torch shim (once) and returns the module-like wrapper."""
-    global _loaded
-    import torch
-
-    _native.lib()  # raises if the core library has not been built
-    if not _loaded:
-        if not _native.TORCH_LIB.exists():
-            raise ImportError(f"{_native.TORCH_LIB} is missing: run `python -m b200_attention_b200.build`")
-        torch.ops.load_library(str(_native.TORCH_LIB))
-        _loaded = True
-    return _KernelModule(spec, torch.ops.b200_attention_b200)
+    return _KernelModule(spec, _native.torch_ops())

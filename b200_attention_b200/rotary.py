@@ -3,7 +3,6 @@ attention call. The reference project has no counterpart (its model's own module
 
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -11,32 +10,6 @@ import torch
 from . import _native as N
 
 HEAD_DIM = 128
-_POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
-
-
-def _check_tokens(name: str, t, like=None) -> None:
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} must be a CUDA tensor (this library has no CPU path)")
-    if t.dtype != torch.bfloat16:
-        raise RuntimeError(f"{name} must be bfloat16, got {t.dtype}")
-    if t.dim() not in (3, 4) or t.size(-1) != HEAD_DIM:
-        raise RuntimeError(f"{name} must be [tokens, heads, {HEAD_DIM}] or [batch, tokens, heads, {HEAD_DIM}], "
-                           f"got {tuple(t.shape)}")
-    if t.stride(-1) != 1:
-        raise RuntimeError(f"{name}: the head_dim axis must be contiguous")
-    if like is not None:
-        if t.device != like.device:
-            raise RuntimeError(f"{name} is on {t.device}, q on {like.device}")
-        if t.dim() != like.dim() or t.shape[:-2] != like.shape[:-2]:
-            raise RuntimeError(f"{name} and q disagree on batch or tokens: {tuple(t.shape)}, {tuple(like.shape)}")
-
-
-def _operand(t: torch.Tensor) -> N.Operand:
-    # (batch, head, token); an axis of one entry is never stepped along
-    stride = [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
-    return N.Operand(t.data_ptr(), stride[0] if t.dim() == 4 else 0, stride[-2], stride[-3])
 
 
 def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -75,6 +48,23 @@ def _dense_apart(t: torch.Tensor) -> bool:
     return True
 
 
+def _check_out(q, k, q_out, k_out) -> None:
+    pairs = [("q", q, q_out)] + ([("k", k, k_out)] if k is not None else [])
+    for name, src, dst in pairs:
+        if not isinstance(dst, torch.Tensor):
+            raise TypeError(f"out of {name} must be a torch.Tensor")
+        if dst.shape != src.shape or dst.dim() < 3:
+            raise RuntimeError(f"out of {name} must match {name} in shape")
+        if not _dense_apart(dst):
+            raise RuntimeError(f"out of {name}: elements share memory")
+    for name, _, dst in pairs:
+        for other, src, _ in pairs:
+            if not (name == other and _same_place(src, dst)) and _may_overlap(src, dst):
+                raise RuntimeError(f"out of {name} overlaps {other} without being it")
+    if k is not None and _may_overlap(q_out, k_out):
+        raise RuntimeError("the outputs overlap")
+
+
 def qk_norm_rope(
     q: torch.Tensor,
     k: Optional[torch.Tensor],
@@ -102,108 +92,29 @@ def qk_norm_rope(
     q_weight, k_weight: [128], both bf16 or both fp32, or None (no norm). Inputs need strides that are multiples of 8
     elements. `out`: tensors to write (may be q and k themselves). One rounding to bf16, at the end. Forward only.
     """
-    _check_tokens("q", q)
-    if k is not None:
-        _check_tokens("k", k, q)
-    elif k_weight is not None:
-        raise RuntimeError("k_weight is given without k")
-    batch, tokens = (q.size(0), q.size(1)) if q.dim() == 4 else (1, q.size(0))
-
-    for name, t in (("positions", positions), ("inv_freq", inv_freq)):
-        if not isinstance(t, torch.Tensor):
+    for name, t, needed in (("q", q, True), ("k", k, False), ("positions", positions, True), ("inv_freq", inv_freq, True),
+                            ("q_weight", q_weight, False), ("k_weight", k_weight, False)):
+        if not isinstance(t, torch.Tensor) and (needed or t is not None):
             raise TypeError(f"{name} must be a torch.Tensor")
-        if t.device != q.device:
-            raise RuntimeError(f"{name} is on {t.device}, q on {q.device}")
-    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float32 or not inv_freq.is_contiguous():
-        raise RuntimeError("inv_freq must be a contiguous fp32 vector")
-    if positions.dtype not in _POSITION_TYPES:
-        raise RuntimeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
-    sections = (inv_freq.numel(),) if sections is None else tuple(int(n) for n in sections)
-    if not 1 <= len(sections) <= 4 or any(n < 0 for n in sections) or not 1 <= sum(sections) <= HEAD_DIM // 2:
-        raise ValueError(f"sections must be 1 to 4 counts that add up to 1 .. {HEAD_DIM // 2}, got {sections}")
+    if sections is None:
+        sections = (inv_freq.numel(),)
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or not 1 <= sum(sections) <= HEAD_DIM // 2:
+        raise ValueError(f"sections must be 1 to 4 counts that add up to 1 .. {HEAD_DIM // 2}, got {tuple(sections)}")
     if inv_freq.numel() != sum(sections):
         raise ValueError(f"inv_freq holds {inv_freq.numel()} frequencies, sections add up to {sum(sections)}")
-    if positions.dim() == 1:
-        positions = positions[None]
-    if positions.dim() == 2 and tuple(positions.shape) == (len(sections), tokens):
-        pos_batch = 0
-    elif positions.dim() == 3 and tuple(positions.shape) == (len(sections), batch, tokens):
-        pos_batch = positions.stride(1)
-    else:
-        raise RuntimeError(f"positions must be [{len(sections)}, {tokens}] or [{len(sections)}, {batch}, {tokens}], "
-                           f"got {tuple(positions.shape)}")
-    weights = [(n, w) for n, w in (("q_weight", q_weight), ("k_weight", k_weight)) if w is not None]
-    for name, w in weights:
-        if not isinstance(w, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if w.device != q.device or tuple(w.shape) != (HEAD_DIM,) or not w.is_contiguous() \
-                or w.dtype not in (torch.bfloat16, torch.float32):
-            raise RuntimeError(f"{name} must be a contiguous bf16 or fp32 vector of {HEAD_DIM} on q's device")
-    if len({w.dtype for _, w in weights}) > 1:
-        raise RuntimeError("q_weight and k_weight must have the same type")
-    if torch.is_grad_enabled():
-        for name, t in [("q", q), ("k", k), ("inv_freq", inv_freq), ("positions", positions)] + weights:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{name} requires grad: this library computes forward passes only")
+    q_out, k_out = (None, None) if out is None else out
     if out is not None:
-        q_out, k_out = out
-        pairs = [("q", q, q_out)] + ([("k", k, k_out)] if k is not None else [])
-        for name, src, dst in pairs:
-            _check_tokens(f"out of {name}", dst, q)
-            if dst.shape != src.shape:
-                raise RuntimeError(f"out of {name} must match {name} in shape")
-            if not _dense_apart(dst):
-                raise RuntimeError(f"out of {name}: elements share memory")
-        for name, _, dst in pairs:
-            for other, src, _ in pairs:
-                if not (name == other and _same_place(src, dst)) and _may_overlap(src, dst):
-                    raise RuntimeError(f"out of {name} overlaps {other} without being it")
-        if k is not None and _may_overlap(q_out, k_out):
-            raise RuntimeError("the outputs overlap")
-
-    def launch():
-        s = torch.cuda.current_stream()
-        if out is None:
-            qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        else:
-            qo, ko = out
-            ko = None if k is None else ko
-        if batch * tokens == 0 or q.size(-2) == 0:
-            return qo, ko
-        a = N.QkNormRopeArgs()
-        a.struct_bytes = C.sizeof(N.QkNormRopeArgs)
-        a.batch, a.tokens, a.heads_q, a.head_dim = batch, tokens, q.size(-2), HEAD_DIM
-        a.q, a.q_out = _operand(q), _operand(qo)
-        if k is not None and k.size(-2) > 0:
-            a.heads_k, a.k, a.k_out = k.size(-2), _operand(k), _operand(ko)
-        a.q_weight = q_weight.data_ptr() if q_weight is not None else None
-        a.k_weight = k_weight.data_ptr() if k_weight is not None else None
-        a.weight_type = int(bool(weights) and weights[0][1].dtype == torch.float32)
-        a.position_type = _POSITION_TYPES[positions.dtype]
-        a.positions = positions.data_ptr()
-        a.position_stride_axis, a.position_stride_batch = positions.stride(0), pos_batch
-        a.position_stride_token = positions.stride(-1)
-        a.inv_freq = inv_freq.data_ptr()
-        a.axes = len(sections)
-        a.section[: len(sections)] = sections
-        a.eps = float(eps)
-        a.interleaved = int(bool(interleaved))
-        a.stream = s.cuda_stream
-        N.check(N.lib().b200attn_qk_norm_rope(C.byref(a)))
-        return qo, ko
-
-    if torch.cuda.current_device() != q.device.index:
-        with torch.cuda.device(q.device):
-            return _on(stream, launch)
-    return _on(stream, launch)
-
-
-def _on(stream, launch):
-    if stream is not None and stream != torch.cuda.current_stream():
+        _check_out(q, k, q_out, k_out)
+    if stream is not None and stream != torch.cuda.current_stream(q.device):
         with torch.cuda.stream(stream):
-            return launch()
-    return launch()
+            return _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out)
+    return _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out)
+
+
+def _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out):
+    qo, ko = N.torch_ops().qk_norm_rope(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out,
+                                        k_out)
+    return qo if q_out is None else q_out, None if k is None else ko if k_out is None else k_out
 
 
 __all__ = ["qk_norm_rope"]
