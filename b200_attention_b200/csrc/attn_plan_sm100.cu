@@ -16,6 +16,11 @@
 // tile (row = token * group + head of the group, which is one TMA box of floor(128 / group) tokens x group
 // heads), so a K/V tile is read once for the whole group, a single token fills `group` rows instead of one,
 // and a block of rows spans fewer tokens and so fewer tiles that the causal diagonal cuts.
+//
+// Pieces of two Q tiles (long prompts, wide batches on a prefix) share every K/V tile, as in the kernel above, and are
+// bound like it by the chain scores -> softmax -> PV of two tiles that fill each other's gaps. A piece of one Q tile
+// (single tokens, short prompts) would run that chain without a partner; so two such pieces run side by side, one on
+// each of the CTA's two lanes, and the K/V ring serves the lanes in turn (LaneWalk).
 
 #include "attn_device_sm100.cuh"
 #include "plan_kernels.cuh"
@@ -43,9 +48,9 @@ enum PlanBarrier : int {
   kPbOFree = 14,     // +q    epilogue (4 warps) -> MMA
   kPbPairFull = 16,  // +slot TMA -> MMA, warp 14
   kPbPairEmpty = 18, // +slot MMA and warp 14 -> TMA
-  kPbTailClean = 20, //       warp 14 -> MMA: the rows of a V tile behind the last key are zero
-  kPbDrain = 21,
-  kNumPlanBarriers = 22
+  kPbTailClean = 20, // +slot warp 14 -> MMA: the rows of a V tile behind the last key are zero
+  kPbDrain = 22,
+  kNumPlanBarriers = 23
 };
 
 struct alignas(16) PlanAux {
@@ -54,29 +59,70 @@ struct alignas(16) PlanAux {
   float row_sum[kQTilesPerItem][kBlockM];
   uint32_t tmem_base;
   uint32_t abort_flag;
-  int32_t piece0, piece1;
+  int32_t first[4];  // pieces of two Q tiles, lane 0's, lane 1's, end; counted in the whole table
   PlanPiece cache[kPieceCache];
 };
 
 constexpr int kPlanSmemBytes = kQTilesPerItem * kTileBytes + kPairSlotsP * kPairBytesP + int(sizeof(PlanAux));
 static_assert(kPlanSmemBytes <= 227 * 1024, "shared memory of a CTA");
 
-// Every role walks the CTA's pieces in the same order.
-struct PlanWalk {
+// The CTA's pieces, counted from its first one: [0, pairs) take both lanes, [pairs, lane1) are lane 0's, [lane1, end)
+// lane 1's. Every role walks them in the same order: the first kind one by one, the others with LaneWalk.
+struct Pieces {
   const PlanAux* aux;
   const PlanPiece* table;
-  int i, n;
-  __device__ __forceinline__ PlanWalk(const PlanParams& p, const PlanAux* a)
-      : aux(a), table(reinterpret_cast<const PlanPiece*>(p.table + kPlanPieceAt) + a->piece0), i(0),
-        n(a->piece1 - a->piece0) {}
-  __device__ __forceinline__ bool take(const PlanPiece*& out) {
-    if (i >= n) return false;
-    out = i < kPieceCache ? &aux->cache[i] : table + i;
-    ++i;
+  int pairs, lane1, end;
+  __device__ __forceinline__ Pieces(const PlanParams& p, const PlanAux* a)
+      : aux(a), table(reinterpret_cast<const PlanPiece*>(p.table + kPlanPieceAt) + a->first[0]),
+        pairs(a->first[1] - a->first[0]), lane1(a->first[2] - a->first[0]), end(a->first[3] - a->first[0]) {}
+  __device__ __forceinline__ const PlanPiece* at(int i) const { return i < kPieceCache ? &aux->cache[i] : table + i; }
+};
+
+// Steps of the pieces of one Q tile: a K/V tile of lane 0, one of lane 1, and so on; a lane that has run out leaves
+// the turns to the other.
+struct LaneWalk {
+  int next[2], end[2], tile[2], tiles[2];
+  int turn;
+  __device__ __forceinline__ explicit LaneWalk(const Pieces& ps) : turn(0) {
+    next[0] = ps.pairs;
+    end[0] = next[1] = ps.lane1;
+    end[1] = ps.end;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      tile[q] = 0;
+      tiles[q] = next[q] < end[q] ? ps.at(next[q])->tiles[0] : 0;
+    }
+  }
+  struct Step {
+    int lane, piece, tile;
+    bool last;  // of its piece
+  };
+  __device__ __forceinline__ bool more() const { return next[0] < end[0] || next[1] < end[1]; }
+  __device__ __forceinline__ bool take(const Pieces& ps, Step& s) {
+    if (!more()) return false;
+    const bool other = turn ? next[1] >= end[1] : next[0] >= end[0];
+    s.lane = other ? turn ^ 1 : turn;
+    turn = s.lane ^ 1;
+    if (s.lane == 0)
+      advance<0>(ps, s);
+    else
+      advance<1>(ps, s);
     return true;
   }
-  __device__ __forceinline__ const PlanPiece* peek() const {
-    return i >= n ? nullptr : (i < kPieceCache ? &aux->cache[i] : table + i);
+  template <int q>
+  __device__ __forceinline__ void advance(const Pieces& ps, Step& s) {
+    s.piece = next[q];
+    s.tile = tile[q];
+    s.last = ++tile[q] == tiles[q];
+    if (s.last) {
+      tile[q] = 0;
+      if (++next[q] < end[q]) tiles[q] = ps.at(next[q])->tiles[0];
+    }
+  }
+  // the piece that follows on a lane whose piece has just had its last step, or null
+  __device__ __forceinline__ const PlanPiece* following(const Pieces& ps, int lane) const {
+    const int n = lane ? next[1] : next[0];
+    return n < (lane ? end[1] : end[0]) ? ps.at(n) : nullptr;
   }
 };
 
@@ -92,7 +138,7 @@ __device__ __forceinline__ int piece_tail(const PlanPiece* pc) {
 __device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const PlanMaps& maps, uint32_t smem_q,
                                uint32_t smem_kv, uint32_t bar0, uint32_t lead, WaitCtx& w) {
   uint32_t slot = 0, empty_parity = 1;  // parity 1 passes on a fresh barrier
-  uint32_t q_empty_parity[kQTilesPerItem] = {1, 1};
+  uint32_t q_empty_parity = 3;           // bit per lane
   uint32_t armed = 0, armed_parity = 0;  // for the early-exit path: "full" barriers armed, last parity of each
   bool ok = true;
   auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
@@ -123,38 +169,56 @@ __device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const Pl
     return true;
   };
 
-  PlanWalk walk(p, aux);
-  const PlanPiece* pc;
-  bool first = true;
-  while (ok && walk.take(pc)) {
-    const int T = piece_tiles(pc);
-    w.item = walk.i - 1;
+  // Q tile `tile` of a piece to a lane: a box of 64 columns x group heads x tile_tokens tokens lands as rows
+  // token * group + head.
+  auto load_q = [&](const PlanPiece* pc, int lane, int tile) -> bool {
+    if (!w.wait_issue(bar(kPbQEmpty + lane), (q_empty_parity >> lane) & 1u, 100 + lane)) return false;
+    q_empty_parity ^= 1u << lane;
+    armed |= 1u << (kPairSlotsP + lane);
+    armed_parity = (armed_parity & ~(1u << (kPairSlotsP + lane))) | (((q_empty_parity >> lane) & 1u) << (kPairSlotsP + lane));
+    const uint32_t full = bar(kPbQFull + lane), dst = smem_q + lane * kTileBytes;
+    const int token = pc->token + tile * p.tile_tokens;
+    mbar_arrive_expect_tx_lead(lead, full, q_bytes);
+    tma_load_4d_lead(lead, dst, &maps.q, 0, 0, pc->kv_head, token, full);
+    tma_load_4d_lead(lead, dst + kBoxBytes, &maps.q, 64, 0, pc->kv_head, token, full);
+    return true;
+  };
+
+  const Pieces ps(p, aux);
+  if (ps.pairs > 0) ok = push_pair(nullptr, 0, ps.at(0), 0, 110);  // the first K tile travels alone
+  for (int n = 0; ok && n < ps.pairs; ++n) {
+    const PlanPiece* pc = ps.at(n);
+    const int T = pc->tiles[1];
+    w.item = n;
     w.tile = 0;
-    if (first) {
-      ok = push_pair(nullptr, 0, pc, 0, 110);  // the first K tile travels alone
-      first = false;
-      if (!ok) break;
-    }
-    for (int q = 0; ok && q < kQTilesPerItem; ++q) {
-      if (pc->tiles[q] == 0) continue;
-      ok = w.wait_issue(bar(kPbQEmpty + q), q_empty_parity[q], 100 + q);
-      if (!ok) break;
-      armed |= 1u << (kPairSlotsP + q);
-      armed_parity = (armed_parity & ~(1u << (kPairSlotsP + q))) | ((q_empty_parity[q] ^ 1u) << (kPairSlotsP + q));
-      q_empty_parity[q] ^= 1u;
-      // box of 64 columns x group heads x tile_tokens tokens: rows land as token * group + head
-      const uint32_t full = bar(kPbQFull + q), dst = smem_q + q * kTileBytes;
-      const int token = pc->token + q * p.tile_tokens;
-      mbar_arrive_expect_tx_lead(lead, full, q_bytes);
-      tma_load_4d_lead(lead, dst, &maps.q, 0, 0, pc->kv_head, token, full);
-      tma_load_4d_lead(lead, dst + kBoxBytes, &maps.q, 64, 0, pc->kv_head, token, full);
-    }
+    for (int q = 0; ok && q < kQTilesPerItem; ++q) ok = load_q(pc, q, q);
     for (int i = 0; ok && i < T; ++i) {
       w.tile = i;
-      if (i + 1 < T) {
-        ok = push_pair(pc, i, pc, i + 1, 111);
+      // the last V with the first K of the CTA's next piece, if any (it is lane 0's, if the pairs end here)
+      const bool last = i + 1 == T;
+      ok = push_pair(pc, i, !last ? pc : n + 1 < ps.end ? ps.at(n + 1) : nullptr, last ? 0 : i + 1, 111);
+    }
+  }
+  if (ok && ps.end > ps.pairs) {
+    LaneWalk walk(ps);
+    const PlanPiece* pc = ps.at(ps.pairs);
+    ok = load_q(pc, 0, 0);
+    if (ok && ps.pairs == 0) ok = push_pair(nullptr, 0, pc, 0, 113);
+    if (ok && ps.lane1 < ps.end) {
+      pc = ps.at(ps.lane1);
+      ok = load_q(pc, 1, 0) && push_pair(nullptr, 0, pc, 0, 114);
+    }
+    LaneWalk::Step st;
+    while (ok && walk.take(ps, st)) {
+      pc = ps.at(st.piece);
+      w.item = st.piece;
+      w.tile = st.tile;
+      if (!st.last) {
+        ok = push_pair(pc, st.tile, pc, st.tile + 1, 115);
       } else {
-        ok = push_pair(pc, i, walk.peek(), 0, 112);  // with the first K of the CTA's next piece, if any
+        const PlanPiece* following = walk.following(ps, st.lane);
+        ok = push_pair(pc, st.tile, following, 0, 116);
+        if (ok && following != nullptr) ok = load_q(following, st.lane, 0);
       }
     }
   }
@@ -190,24 +254,33 @@ __device__ void plan_tail_role(const PlanParams& p, const PlanAux* aux, uint8_t*
     }
     __syncwarp();
     if (lane == 0) {
-      if (tail > 0) mbar_arrive(bar(kPbTailClean));
+      if (tail > 0) mbar_arrive(bar(kPbTailClean + slot));
       mbar_arrive(bar(kPbPairEmpty + slot));
     }
     slot ^= 1u;
     if (slot == 0) full_parity ^= 1u;
     return true;
   };
-  PlanWalk walk(p, aux);
-  const PlanPiece* pc;
-  bool first = true;
-  while (walk.take(pc)) {
-    const int T = piece_tiles(pc);
-    w.item = walk.i - 1;
-    if (first && !next_pair(0)) return;
-    first = false;
+  const Pieces ps(p, aux);
+  if (ps.pairs > 0 && !next_pair(0)) return;
+  for (int n = 0; n < ps.pairs; ++n) {
+    const PlanPiece* pc = ps.at(n);
+    const int T = pc->tiles[1];
+    w.item = n;
     for (int i = 0; i < T; ++i) {
       w.tile = i;
       if (!next_pair(i + 1 == T ? piece_tail(pc) : 0)) return;
+    }
+  }
+  if (ps.end > ps.pairs) {
+    if (ps.pairs == 0 && !next_pair(0)) return;
+    if (ps.lane1 < ps.end && !next_pair(0)) return;
+    LaneWalk walk(ps);
+    LaneWalk::Step st;
+    while (walk.take(ps, st)) {
+      w.item = st.piece;
+      w.tile = st.tile;
+      if (!next_pair(st.last ? piece_tail(ps.at(st.piece)) : 0)) return;
     }
   }
 }
@@ -216,39 +289,63 @@ __device__ void plan_tail_role(const PlanParams& p, const PlanAux* aux, uint8_t*
 __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t smem_q, uint32_t smem_kv,
                               uint32_t bar0, uint32_t tmem_base, uint32_t lead, WaitCtx& w) {
   auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
-  uint32_t slot = 0, full_parity = 0, tail_parity = 0;
-  uint32_t q_full_parity[kQTilesPerItem] = {0, 0}, p_parity[kQTilesPerItem] = {0, 0};
-  uint32_t o_free_parity[kQTilesPerItem] = {1, 1};  // passes on the fresh barrier: both accumulators start out free
+  uint32_t slot = 0, full_parity = 0;
+  uint32_t tail_parity = 0;      // bit per slot
+  uint32_t q_full_parity = 0, p_parity = 0;  // bit per lane
+  uint32_t o_free_parity = 3;    // passes on the fresh barrier: both accumulators start out free
   bool ok = true, k_ready = false;
 
-  PlanWalk walk(p, aux);
-  const PlanPiece* pc;
-  while (ok && walk.take(pc)) {
+  auto wait_pair = [&](int site) -> bool {
+    if (!w.wait_issue(bar(kPbPairFull + slot), full_parity, site)) return false;
+    slot ^= 1u;
+    if (slot == 0) full_parity ^= 1u;
+    return true;  // the pair is the one in slot ^ 1
+  };
+  // First scores of a piece on a lane, K in the pair waited for last.
+  auto first_scores = [&](int lane, int tiles) -> bool {
+    if (!w.wait_issue(bar(kPbQFull + lane), (q_full_parity >> lane) & 1u, 201 + lane)) return false;
+    q_full_parity ^= 1u << lane;
+    tc_fence_after_sync();
+    issue_qk(lead, tmem_base + lane * kBlockN, smem_q + lane * kTileBytes, smem_kv + (slot ^ 1u) * kPairBytesP + kTileBytes);
+    umma_commit_lead(lead, bar(kPbSFull + lane));
+    if (tiles == 1) umma_commit_lead(lead, bar(kPbQEmpty + lane));
+    return true;
+  };
+  // The V tile of the pair waited for last, if a piece's keys end inside it, once its other rows are zero.
+  auto wait_tail = [&]() -> bool {
+    const uint32_t s = slot ^ 1u;
+    if (!w.wait_issue(bar(kPbTailClean + s), (tail_parity >> s) & 1u, 211)) return false;
+    tail_parity ^= 1u << s;
+    return true;
+  };
+  // PV of tile i on a lane, once its probabilities are there and, for the first tile, its accumulator has been read
+  // out by the epilogue of the piece before.
+  auto weighted_sum = [&](int lane, int i, uint32_t v_smem) -> bool {
+    if (i == 0) {
+      if (!w.wait_issue(bar(kPbOFree + lane), (o_free_parity >> lane) & 1u, 240 + lane)) return false;
+      o_free_parity ^= 1u << lane;
+    }
+    if (!w.wait_issue(bar(kPbPReady + lane), (p_parity >> lane) & 1u, 220 + lane)) return false;
+    p_parity ^= 1u << lane;
+    tc_fence_after_sync();
+    issue_pv(lead, tmem_base + kQTilesPerItem * kBlockN + lane * kHeadDim, tmem_base + lane * kBlockN, v_smem, i > 0);
+    return true;
+  };
+
+  const Pieces ps(p, aux);
+  for (int n = 0; ok && n < ps.pairs; ++n) {
+    const PlanPiece* pc = ps.at(n);
     const int Tq[kQTilesPerItem] = {pc->tiles[0], pc->tiles[1]};
-    const int T = max(Tq[0], Tq[1]);
+    const int T = Tq[1];
     const bool tail = piece_tail(pc) > 0;
-    w.item = walk.i - 1;
+    w.item = n;
     w.tile = 0;
     if (!k_ready) {
-      if (!(ok = w.wait_issue(bar(kPbPairFull + slot), full_parity, 200))) break;
-      slot ^= 1u;
-      if (slot == 0) full_parity ^= 1u;
+      if (!(ok = wait_pair(200))) break;
       k_ready = true;
     }
-    {
-      const uint32_t k_smem = smem_kv + (slot ^ 1u) * kPairBytesP + kTileBytes;
 #pragma unroll
-      for (int q = 0; q < kQTilesPerItem; ++q) {
-        if (Tq[q] > 0) {
-          if (!(ok = w.wait_issue(bar(kPbQFull + q), q_full_parity[q], 201 + q))) break;
-          q_full_parity[q] ^= 1u;
-          tc_fence_after_sync();
-          issue_qk(lead, tmem_base + q * kBlockN, smem_q + q * kTileBytes, k_smem);
-          umma_commit_lead(lead, bar(kPbSFull + q));
-          if (Tq[q] == 1) umma_commit_lead(lead, bar(kPbQEmpty + q));
-        }
-      }
-    }
+    for (int q = 0; q < kQTilesPerItem; ++q) ok = ok && first_scores(q, Tq[q]);
     if (!ok) break;
     // also covers the PV of the previous piece that read the V half of this pair
     umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
@@ -256,32 +353,16 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
     for (int i = 0; ok && i < T; ++i) {
       w.tile = i;
       // V_i and K_{i+1} (or K_0 of this CTA's next piece) in one phase
-      if (!(ok = w.wait_issue(bar(kPbPairFull + slot), full_parity, 210))) break;
-      const uint32_t v_smem = smem_kv + slot * kPairBytesP;
+      if (!(ok = wait_pair(210))) break;
+      const uint32_t v_smem = smem_kv + (slot ^ 1u) * kPairBytesP;
       const uint32_t k_smem = v_smem + kTileBytes;
-      const uint32_t pair_empty = bar(kPbPairEmpty + slot);
-      slot ^= 1u;
-      if (slot == 0) full_parity ^= 1u;
-      if (tail && i + 1 == T) {
-        if (!(ok = w.wait_issue(bar(kPbTailClean), tail_parity, 211))) break;
-        tail_parity ^= 1u;
-      }
+      if (tail && i + 1 == T && !(ok = wait_tail())) break;
 #pragma unroll
       for (int q = 0; q < kQTilesPerItem; ++q) {
         if (i < Tq[q]) {
-          const uint32_t s_tmem = tmem_base + q * kBlockN;
-          const uint32_t o_tmem = tmem_base + kQTilesPerItem * kBlockN + q * kHeadDim;
-          if (i == 0) {
-            // the previous piece's epilogue must have read O_q out before it is overwritten
-            if (!(ok = w.wait_issue(bar(kPbOFree + q), o_free_parity[q], 240 + q))) break;
-            o_free_parity[q] ^= 1u;
-          }
-          if (!(ok = w.wait_issue(bar(kPbPReady + q), p_parity[q], 220 + q))) break;
-          tc_fence_after_sync();
-          issue_pv(lead, o_tmem, s_tmem, v_smem, /*accumulate=*/i > 0);
-          p_parity[q] ^= 1u;
+          if (!(ok = weighted_sum(q, i, v_smem))) break;
           if (i + 1 < Tq[q]) {
-            issue_qk(lead, s_tmem, smem_q + q * kTileBytes, k_smem);
+            issue_qk(lead, tmem_base + q * kBlockN, smem_q + q * kTileBytes, k_smem);
             umma_commit_lead(lead, bar(kPbSFull + q));
             if (i + 2 == Tq[q]) umma_commit_lead(lead, bar(kPbQEmpty + q));
           } else {
@@ -289,7 +370,39 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
           }
         }
       }
-      if (ok && i + 1 < T) umma_commit_lead(lead, pair_empty);
+      if (ok && i + 1 < T) umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
+    }
+  }
+  if (ok && ps.end > ps.pairs) {
+    LaneWalk walk(ps);
+    if (!k_ready) ok = wait_pair(203);
+    ok = ok && first_scores(0, walk.tiles[0]);
+    if (ok) umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
+    if (ok && ps.lane1 < ps.end) {
+      ok = wait_pair(204) && first_scores(1, walk.tiles[1]);
+      if (ok) umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
+    }
+    LaneWalk::Step st;
+    while (ok && walk.take(ps, st)) {
+      w.item = st.piece;
+      w.tile = st.tile;
+      const int lane = st.lane;
+      if (!(ok = wait_pair(212))) break;
+      const uint32_t v_smem = smem_kv + (slot ^ 1u) * kPairBytesP;
+      if (st.last && piece_tail(ps.at(st.piece)) > 0 && !(ok = wait_tail())) break;
+      if (!(ok = weighted_sum(lane, st.tile, v_smem))) break;
+      if (!st.last) {
+        issue_qk(lead, tmem_base + lane * kBlockN, smem_q + lane * kTileBytes, v_smem + kTileBytes);
+        umma_commit_lead(lead, bar(kPbSFull + lane));
+        const int tiles = lane ? walk.tiles[1] : walk.tiles[0];
+        if (st.tile + 2 == tiles) umma_commit_lead(lead, bar(kPbQEmpty + lane));
+      } else {
+        umma_commit_lead(lead, bar(kPbPvDone + lane));
+        const PlanPiece* following = walk.following(ps, lane);
+        if (following != nullptr && !(ok = first_scores(lane, following->tiles[0]))) break;
+      }
+      // nobody waits for the last pair to be handed back, and the CTA may be gone by then
+      if (walk.more()) umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
     }
   }
 
@@ -316,24 +429,27 @@ __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t ba
   const uint32_t p_tmem = s_tmem;  // bf16 P overwrites S columns 0..63
   const uint32_t o_tmem = tmem_base + kQTilesPerItem * kBlockN + q * kHeadDim + lane_field;
   const int r = warp_in_group * 32 + lane;
-  const int my_token = q * p.tile_tokens + min(r, p.tile_rows - 1) / p.group;  // of the block; idle rows go with the last
+  const int token_in_tile = min(r, p.tile_rows - 1) / p.group;  // idle rows go with the last
   const float scale_log2 = p.scale_log2;
   const f2 scale2 = f2_splat(scale_log2);
   uint32_t s_parity = 0, fin_free_parity = 1;
 
-  PlanWalk walk(p, aux);
-  const PlanPiece* pc;
-  while (walk.take(pc)) {
-    const int T = pc->tiles[q];
-    if (T == 0) continue;
-    const int n_keys = pc->n_keys, diag = pc->diag;
+  const Pieces ps(p, aux);
+  const int my_end = q ? ps.end : ps.lane1;
+  for (int n = 0; n < my_end; ++n) {
+    if (q && n == ps.pairs) n = ps.lane1;  // over lane 0's pieces
+    if (n >= my_end) break;
+    const PlanPiece* pc = ps.at(n);
+    const int tile = n < ps.pairs ? q : 0;  // which of the piece's Q tiles
+    const int T = pc->tiles[tile];
+    const int n_keys = pc->n_keys, diag = pc->diag + tile * p.tile_tokens;
     // rows of this tile that exist; a warp without one only keeps the protocol going
-    const int rows = (min(pc->n_tokens - q * p.tile_tokens, p.tile_tokens)) * p.group;
+    const int rows = (min(pc->n_tokens - tile * p.tile_tokens, p.tile_tokens)) * p.group;
     const bool row_live = r < rows;
     const bool warp_live = warp_in_group * 32 < rows;
-    const int tile_limit = min(n_keys - 1, diag + q * p.tile_tokens);  // last key that the tile's first row sees
-    const int row_limit = min(n_keys - 1, diag + my_token);            // last key that this row sees
-    w.item = walk.i - 1;
+    const int tile_limit = min(n_keys - 1, diag);                 // last key that the tile's first row sees
+    const int row_limit = min(n_keys - 1, diag + token_in_tile);  // last key that this row sees
+    w.item = n;
     w.tile = 0;
     if (!w.wait_warp(bar(kPbFinFree + q), fin_free_parity, 310 + q)) return;
     fin_free_parity ^= 1u;
@@ -427,24 +543,19 @@ __device__ void plan_epilogue_role(const PlanParams& p, const PlanAux* aux, uint
   const uint32_t lane_field = uint32_t(warp_in_group * 32) << 16;
   const int r = warp_in_group * 32 + lane;
   const int token_in_tile = r / p.group, head_in_group = r - token_in_tile * p.group;
-  uint32_t fin_parity[kQTilesPerItem] = {0, 0};
+  uint32_t fin_parity = 0;  // bit per lane
 
-  PlanWalk walk(p, aux);
-  const PlanPiece* pc;
-  while (walk.take(pc)) {
-    w.item = walk.i - 1;
-    for (int q = 0; q < kQTilesPerItem; ++q) {
-      if (pc->tiles[q] == 0) continue;
-      w.tile = pc->tiles[q];
-      if (!w.wait_warp(bar(kPbFin + q), fin_parity[q], 410 + q)) return;
-      if (!w.wait_warp(bar(kPbPvDone + q), fin_parity[q], 420 + q)) return;
-      fin_parity[q] ^= 1u;
+  // The result of a lane's piece: its Q tile `tile` of the piece.
+  auto finish = [&](const PlanPiece* pc, int q, int tile) -> bool {
+      if (!w.wait_warp(bar(kPbFin + q), (fin_parity >> q) & 1u, 410 + q)) return false;
+      if (!w.wait_warp(bar(kPbPvDone + q), (fin_parity >> q) & 1u, 420 + q)) return false;
+      fin_parity ^= 1u << q;
       tc_fence_after_sync();
       const float m = aux->row_max[q][r];
       const float l = aux->row_sum[q][r];
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kPbFinFree + q));
-      const int token = q * p.tile_tokens + token_in_tile;  // of the block
+      const int token = tile * p.tile_tokens + token_in_tile;  // of the block
       const bool live = r < p.tile_rows && token < pc->n_tokens;
       const bool any_live = __any_sync(0xffffffffu, live);
       const bool seen = l != 0.0f;  // false: the row saw no key (a NaN sum counts as seen)
@@ -494,7 +605,25 @@ __device__ void plan_epilogue_role(const PlanParams& p, const PlanAux* aux, uint
       tc_fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kPbOFree + q));
+      return true;
+  };
+
+  const Pieces ps(p, aux);
+  for (int n = 0; n < ps.pairs; ++n) {
+    const PlanPiece* pc = ps.at(n);
+    w.item = n;
+    for (int q = 0; q < kQTilesPerItem; ++q) {
+      w.tile = pc->tiles[q];
+      if (!finish(pc, q, q)) return;
     }
+  }
+  LaneWalk walk(ps);  // pieces end in the order of their last steps
+  LaneWalk::Step st;
+  while (walk.take(ps, st)) {
+    if (!st.last) continue;
+    w.item = st.piece;
+    w.tile = st.tile;
+    if (!finish(ps.at(st.piece), st.lane, 0)) return;
   }
 }
 
@@ -516,12 +645,15 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
   w.tile = -1;
 
   const bool misaligned = (smem_q & 1023u) != 0;  // uniform across the CTA
-  const int piece0 = p.table[kPlanCtaAt + blockIdx.x], piece1 = p.table[kPlanCtaAt + blockIdx.x + 1];
+  const int4 first = reinterpret_cast<const int4*>(p.table + kPlanCtaAt)[blockIdx.x];
+  const int piece0 = first.x, piece1 = first.w;
   if (piece0 >= piece1) return;  // uniform across the CTA: a table with fewer CTAs than the grid
   if (threadIdx.x == 0) {
     aux->abort_flag = 0;
-    aux->piece0 = piece0;
-    aux->piece1 = piece1;
+    aux->first[0] = first.x;
+    aux->first[1] = first.y;
+    aux->first[2] = first.z;
+    aux->first[3] = first.w;
     if (misaligned) {
       w.raise(kDevSmemMisaligned, 3, 0);
     } else {
@@ -538,8 +670,8 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
       for (int s = 0; s < kPairSlotsP; ++s) {
         mbar_init(bar0 + 8u * (kPbPairFull + s), 1);
         mbar_init(bar0 + 8u * (kPbPairEmpty + s), 2);
+        mbar_init(bar0 + 8u * (kPbTailClean + s), 1);
       }
-      mbar_init(bar0 + 8u * kPbTailClean, 1);
       mbar_init(bar0 + 8u * kPbDrain, 1);
       mbar_init_fence();
       fence_proxy_async_smem();

@@ -19,11 +19,15 @@ namespace {
 
 constexpr int kTile = 128;
 
-// Costs in thousandths of a K/V tile with two Q tiles on the tensor cores.
-constexpr int64_t kTilePair = 1000;    // two Q tiles against one K/V tile
-constexpr int64_t kTileSingle = 800;   // one Q tile: the same chain of steps without overlap
-constexpr int64_t kPieceStart = 1500;  // Q load, first scores, last PV, stores
-constexpr int64_t kJoin = 2500;        // the second kernel, once
+// Costs in thousandths of the time of a K/V tile against two Q tiles (about 1.6 us). A piece of one Q tile runs on
+// one of a CTA's two lanes: alone it is bound by its chain of steps, beside another lane by what the two share.
+constexpr int64_t kTilePair = 1000;
+constexpr int64_t kPairStart = 1500;    // Q load, first scores, last PV, stores
+constexpr int64_t kTileShared = 600;    // tensor pipe and memory, per tile of a lane
+constexpr int64_t kSharedStart = 500;
+constexpr int64_t kTileChain = 850;     // scores, softmax, PV of one tile after the other
+constexpr int64_t kChainStart = 1200;
+constexpr int64_t kJoin = 2500;         // the second kernel, once
 
 struct Item {
   int32_t token, n_tokens, kv_row, n_keys, tiles0, tiles1, diag, kv_head, source;
@@ -31,8 +35,14 @@ struct Item {
   int32_t longest() const { return tiles1 > 0 ? tiles1 : tiles0; }
 };
 
-int64_t cost_of(int32_t tiles0, int32_t tiles1) {
-  return kPieceStart + (tiles1 > 0 ? int64_t(tiles1) * kTilePair : int64_t(tiles0) * kTileSingle);
+struct Cost {
+  bool pair;
+  int64_t shared;  // of the CTA's time
+  int64_t chain;   // of a lane's time, for one Q tile
+};
+Cost cost_of(const PlanPiece& p) {
+  if (p.tiles[1] > 0) return {true, kPairStart + p.tiles[1] * kTilePair, 0};
+  return {false, kSharedStart + p.tiles[0] * kTileShared, kChainStart + p.tiles[0] * kTileChain};
 }
 
 // Piece `c` of an item cut every `len` tiles.
@@ -60,13 +70,50 @@ int32_t even_len(const Item& it, int32_t len) {
   return (it.longest() + n - 1) / n;
 }
 
-using Load = std::pair<int64_t, int32_t>;  // (busy until, CTA)
-using LoadQueue = std::priority_queue<Load, std::vector<Load>, std::greater<Load>>;
+// Deals pieces (longest first, in the order given) to the CTA that is free first, and pieces of one Q tile to the
+// lane of it that is. Returns when the last CTA finishes.
+struct Dealer {
+  using Load = std::pair<int64_t, int32_t>;  // (busy until, CTA)
+  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> free;
+  struct Cta {
+    int64_t pairs = 0, shared = 0, lane[2] = {0, 0};
+    int64_t end() const { return pairs + std::max(shared, std::max(lane[0], lane[1])); }
+  };
+  std::vector<Cta> cta;
+  explicit Dealer(int32_t ctas) : cta(size_t(ctas)) {
+    std::vector<Load> v(cta.size());
+    for (size_t c = 0; c < v.size(); ++c) v[c] = {0, int32_t(c)};
+    free = decltype(free)(std::greater<Load>(), std::move(v));
+  }
+  struct Place {
+    int32_t cta, lane;
+  };
+  Place deal(const Cost& c) {
+    const int32_t at = free.top().second;
+    free.pop();
+    Cta& t = cta[size_t(at)];
+    int32_t lane = 0;
+    if (c.pair) {
+      t.pairs += c.shared;
+    } else {
+      lane = t.lane[1] < t.lane[0] ? 1 : 0;
+      t.lane[lane] += c.chain;
+      t.shared += c.shared;
+    }
+    // by the shared time: a CTA with one busy lane takes a second piece almost for nothing
+    free.push({t.pairs + std::max(t.shared, std::min(t.lane[0], t.lane[1])), at});
+    return {at, lane};
+  }
+  int64_t end() const {
+    int64_t e = 0;
+    for (const Cta& t : cta) e = std::max(e, t.end());
+    return e;
+  }
+};
 
-LoadQueue empty_loads(int32_t ctas) {
-  std::vector<Load> v(static_cast<size_t>(ctas));
-  for (int32_t c = 0; c < ctas; ++c) v[size_t(c)] = {0, c};
-  return LoadQueue(std::greater<Load>(), std::move(v));
+bool longer(const Cost& a, const Cost& b) {
+  if (a.pair != b.pair) return a.pair;  // pieces of two Q tiles come first on every CTA
+  return a.shared > b.shared;
 }
 
 }  // namespace
@@ -165,34 +212,33 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   int32_t best_len = std::max(longest, 1);
   if (!items.empty()) {
     std::vector<int32_t> lens{std::max(longest, 1)};
-    const int64_t even = (total_tiles + in.sm_count - 1) / in.sm_count;
-    for (const int64_t parts : {1, 2, 3, 4, 6, 8}) {
-      const int64_t len = std::max<int64_t>(2, (even + parts - 1) / parts);
+    auto consider = [&](int64_t len) {
+      len = std::max<int64_t>(2, len);
       if (len < longest && std::find(lens.begin(), lens.end(), int32_t(len)) == lens.end()) lens.push_back(int32_t(len));
+    };
+    const int64_t even = (total_tiles + in.sm_count - 1) / in.sm_count;
+    for (const int64_t parts : {1, 2, 3, 4, 6, 8}) consider((even + parts - 1) / parts);
+    // as many pieces of the longest items as fill the CTAs, or their lanes, a whole number of times
+    int64_t long_items = 0;
+    for (const Item& it : items) long_items += 2 * it.longest() > longest ? 1 : 0;
+    for (const int64_t rounds : {1, 2, 3, 4, 6}) {
+      const int64_t n = rounds * in.sm_count / long_items;
+      if (n > 1) consider((longest + n - 1) / n);
     }
     int64_t best = -1;
-    std::vector<int64_t> costs;
+    std::vector<Cost> costs;
     for (const int32_t len : lens) {
       costs.clear();
       bool any_cut = has_prefix;
       for (const Item& it : items) {
         const int32_t n = cuts_of(it, len), l = even_len(it, len);
         any_cut = any_cut || n > 1;
-        for (int32_t c = 0; c < n; ++c) {
-          const PlanPiece p = cut_piece(it, c * l, std::min(l, it.longest() - c * l));
-          costs.push_back(cost_of(p.tiles[0], p.tiles[1]));
-        }
+        for (int32_t c = 0; c < n; ++c) costs.push_back(cost_of(cut_piece(it, c * l, std::min(l, it.longest() - c * l))));
       }
-      std::sort(costs.begin(), costs.end(), std::greater<int64_t>());
-      LoadQueue q = empty_loads(in.sm_count);
-      int64_t end = 0;
-      for (const int64_t c : costs) {
-        const Load l = q.top();
-        q.pop();
-        q.push({l.first + c, l.second});
-        end = std::max(end, l.first + c);
-      }
-      end += any_cut ? kJoin : 0;
+      std::sort(costs.begin(), costs.end(), longer);
+      Dealer dealer(in.sm_count);
+      for (const Cost& c : costs) dealer.deal(c);
+      const int64_t end = dealer.end() + (any_cut ? kJoin : 0);
       if (best < 0 || end < best) {
         best = end;
         best_len = len;
@@ -203,7 +249,7 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   // ---- pieces, with the rows of their partial results
   struct Piece {
     PlanPiece p;
-    int64_t cost;
+    Cost cost;
     int32_t head_group;
   };
   // K/V of sixteen heads at a time where all of it would not stay in L2 (see CausalWalk's groups)
@@ -223,7 +269,7 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
         slots += int64_t(it.n_tokens) * group;
         if (slots >= (int64_t(1) << 31) - 512) return "too many partial rows";
       }
-      p.cost = cost_of(p.p.tiles[0], p.p.tiles[1]);
+      p.cost = cost_of(p.p);
       p.head_group = by_groups ? it.kv_head / 16 : 0;
       pieces.push_back(p);
     }
@@ -284,20 +330,20 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   for (size_t i = 0; i < order.size(); ++i) order[i] = int32_t(i);
   std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) {
     const Piece &x = pieces[size_t(a)], &y = pieces[size_t(b)];
-    if (x.head_group != y.head_group) return x.head_group < y.head_group;
-    return x.cost > y.cost;
+    if (x.cost.pair == y.cost.pair && x.head_group != y.head_group) return x.head_group < y.head_group;
+    return longer(x.cost, y.cost);
   });
-  std::vector<std::vector<int32_t>> dealt(size_t(in.sm_count));
-  LoadQueue q = empty_loads(in.sm_count);
+  std::vector<std::vector<int32_t>> dealt(size_t(in.sm_count) * 3);  // pairs, lane 0, lane 1 of each CTA
+  Dealer dealer(in.sm_count);
   for (const int32_t i : order) {
-    const Load l = q.top();
-    q.pop();
-    dealt[size_t(l.second)].push_back(i);
-    q.push({l.first + pieces[size_t(i)].cost, l.second});
+    const Cost& c = pieces[size_t(i)].cost;
+    const Dealer::Place at = dealer.deal(c);
+    dealt[size_t(at.cta) * 3 + size_t(c.pair ? 0 : 1 + at.lane)].push_back(i);
   }
   plan->grid = 0;
   for (int32_t c = 0; c < in.sm_count; ++c)
-    if (!dealt[size_t(c)].empty()) plan->grid = c + 1;
+    for (int32_t k = 0; k < 3; ++k)
+      if (!dealt[size_t(c) * 3 + size_t(k)].empty()) plan->grid = c + 1;
 
   // ---- table
   const size_t unit_at = size_t(kPlanPieceAt) + pieces.size() * (sizeof(PlanPiece) / 4);
@@ -311,10 +357,13 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   t[kPlanHdrPartAt] = int32_t(part_at);
   PlanPiece* out = reinterpret_cast<PlanPiece*>(t + kPlanPieceAt);
   int32_t k = 0;
-  for (int32_t c = 0; c <= kPlanMaxCtas; ++c) {
-    t[kPlanCtaAt + c] = k;
-    if (c < in.sm_count)
-      for (const int32_t i : dealt[size_t(c)]) out[k++] = pieces[size_t(i)].p;
+  for (int32_t c = 0; c < kPlanMaxCtas; ++c) {
+    for (int32_t part = 0; part < 3; ++part) {
+      t[kPlanCtaAt + 4 * c + part] = k;
+      if (c < in.sm_count)
+        for (const int32_t i : dealt[size_t(c) * 3 + size_t(part)]) out[k++] = pieces[size_t(i)].p;
+    }
+    t[kPlanCtaAt + 4 * c + 3] = k;
   }
   std::copy(units.begin(), units.end(), reinterpret_cast<PlanUnit*>(t + unit_at));
   std::copy(parts.begin(), parts.end(), t + part_at);

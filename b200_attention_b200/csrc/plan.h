@@ -8,15 +8,18 @@
 
 namespace b200attn {
 
-// A piece: up to two Q tiles of packed rows against a run of 128-key K/V tiles of one K/V head.
+// A piece: one or two Q tiles of packed rows against a run of 128-key K/V tiles of one K/V head.
 // Query heads that share a K/V head are packed into the rows of a tile: row r of a tile is token
 // r / group, head r % group of the group, so a tile holds floor(128 / group) tokens.
+// A CTA has two lanes, each with a Q tile, scores and an accumulator of its own. A piece of two Q
+// tiles takes both, and they share every K/V tile. Pieces of one Q tile are walked two at a time,
+// one on each lane, with K/V tiles fetched for the lanes in turn.
 struct alignas(16) PlanPiece {
   int32_t token;     // first token (row of q and o)
   int32_t n_tokens;  // tokens of this block, 1 .. 2 * floor(128 / group)
   int32_t kv_row;    // first key: row of k and v (of the prefix's, if source == 1)
   int32_t n_keys;    // keys from kv_row on that belong to this piece
-  int32_t tiles[2];  // K/V tiles that each Q tile visits; [0] >= 1, [1] == 0 or >= [0]
+  int32_t tiles[2];  // K/V tiles that each Q tile visits; [0] >= 1, [1] >= [0], or 0: one Q tile
   int32_t diag;      // token i of the block sees keys j <= diag + i, j counted from kv_row
   int32_t kv_head;
   int32_t source;    // 0: k and v, 1: the prefix's
@@ -33,13 +36,13 @@ struct alignas(16) PlanUnit {
 };
 static_assert(sizeof(PlanUnit) == 32, "table layout");
 
-// The table as the kernels see it, in 32-bit words: header, first piece of every CTA, pieces,
-// units, parts (the row of the partials that holds the unit's first token, head 0 of the group).
+// The table as the kernels see it, in 32-bit words: header, the pieces of every CTA as four bounds
+// (pieces of two Q tiles, then lane 0's, then lane 1's, end), pieces, units, parts (the row of the partials that holds the unit's first token, head 0 of the group).
 constexpr int kPlanMaxCtas = 160;
-constexpr int kPlanMagic = 0x62706c31;
+constexpr int kPlanMagic = 0x62706c32;
 enum PlanHeader : int { kPlanHdrMagic = 0, kPlanHdrPieces, kPlanHdrUnits, kPlanHdrUnitAt, kPlanHdrPartAt, kPlanHeaderWords = 16 };
 constexpr int kPlanCtaAt = kPlanHeaderWords;
-constexpr int kPlanPieceAt = kPlanCtaAt + ((kPlanMaxCtas + 1 + 3) / 4) * 4;
+constexpr int kPlanPieceAt = kPlanCtaAt + 4 * kPlanMaxCtas;
 
 constexpr int kPlanJoinRows = 32;  // most rows of a join unit (one token at least)
 constexpr int32_t kPlanNoDiag = 1 << 30;

@@ -11,7 +11,7 @@ import torch
 from b200_attention_b200 import _native as N
 from b200_attention_b200 import ops, packed
 
-CTA_AT, PIECE_AT = 16, 180  # words: first piece of each CTA, pieces
+CTA_AT, PIECE_AT = 16, 656  # words: bounds of each CTA's pieces (two Q tiles, lane 0, lane 1, end), pieces
 
 
 def expand(lens_q, lens_kv, heads, heads_kv, *, causal, starts=None, prefix=0, sm_count=0):
@@ -21,13 +21,18 @@ def expand(lens_q, lens_kv, heads, heads_kv, *, causal, starts=None, prefix=0, s
     t, info = s.table.numpy(), s.info
     group = heads // heads_kv
     per_tile = 128 // group
-    ctas = t[CTA_AT:CTA_AT + 161]
-    assert ctas[0] == 0 and ctas[-1] == info.pieces == t[1] and (np.diff(ctas) >= 0).all()
-    assert (np.diff(ctas)[info.grid:] == 0).all() and info.grid <= (sm_count or 148)
+    ctas = t[CTA_AT:PIECE_AT].reshape(160, 4)
+    assert ctas[0, 0] == 0 and ctas[-1, 3] == info.pieces == t[1] and (np.diff(ctas.ravel()) >= 0).all()
+    assert (ctas[1:, 0] == ctas[:-1, 3]).all()
+    assert (ctas[info.grid:, 0] == info.pieces).all() and info.grid <= (sm_count or 148)
     assert info.workspace_bytes == info.slot_rows * 129 * 4 and info.table_bytes == 4 * t.size
     pieces = t[PIECE_AT:PIECE_AT + 12 * info.pieces].reshape(-1, 12)
     units = t[t[3]:t[3] + 8 * info.units].reshape(-1, 8)
     parts = t[t[4]:]
+    both = pieces[:, 5] > 0
+    for pairs, lane0, lane1, end in ctas.tolist():
+        assert both[pairs:lane0].all() and not both[lane0:end].any()
+        assert lane1 > lane0 or end == lane1, "lane 1 has work, lane 0 none"
     runs, slot_owner = {}, {}
     for token, n, row, keys, tiles0, tiles1, diag, head, source, slot in pieces[:, :10].tolist():
         assert 1 <= n <= 2 * per_tile and keys > 0 and tiles0 >= 1
@@ -124,7 +129,8 @@ def test_work_is_spread_evenly(native_built):
         s = packed.Schedule(lens_q, lens_kv, heads=heads, heads_kv=heads_kv)
         t = s.table.numpy()
         pieces = t[PIECE_AT:PIECE_AT + 12 * s.info.pieces].reshape(-1, 12)
-        tiles = [pieces[a:b, 4:6].max(1).sum() for a, b in zip(t[CTA_AT:CTA_AT + 148], t[CTA_AT + 1:CTA_AT + 149])]
+        ctas = t[CTA_AT:PIECE_AT].reshape(160, 4)
+        tiles = [pieces[a:b, 4:6].max(1).sum() for a, b in ctas[:148, [0, 3]]]
         assert max(tiles) <= 1.15 * np.mean(tiles) + 3
 
 
