@@ -20,7 +20,10 @@
 // Pieces of two Q tiles (long prompts, wide batches on a prefix) share every K/V tile, as in the kernel above, and are
 // bound like it by the chain scores -> softmax -> PV of two tiles that fill each other's gaps. A piece of one Q tile
 // (single tokens, short prompts) would run that chain without a partner; so two such pieces run side by side, one on
-// each of the CTA's two lanes, and the K/V ring serves the lanes in turn (LaneWalk).
+// each of the CTA's two lanes, and the K/V ring serves the lanes in turn (LaneWalk). Where such pieces have at most
+// 32 rows, a lane's Q buffer holds four of them and their loads run ahead, so that a lane goes from piece to piece
+// without waiting for Q. (The tensor cores read 128 rows from there: rows that are not the piece's own give scores
+// that nobody looks at.)
 
 #include "attn_device_sm100.cuh"
 #include "plan_kernels.cuh"
@@ -32,25 +35,27 @@ namespace {
 constexpr int kPairSlotsP = 2;
 constexpr int kPairBytesP = 2 * kTileBytes;
 constexpr int kPlanThreads = 512;
-constexpr int kPlanRegsSoftmax = 192;
+constexpr int kPlanRegsSoftmax = 184;
 constexpr int kPlanRegsEpilogue = 64;
-constexpr int kPlanRegsOther = 64;
+constexpr int kPlanRegsOther = 80;
+constexpr int kQSlots = 4;        // small Q tiles that a lane's buffer holds
+constexpr int kQSlotRows = 32;    // rows of each
 constexpr int kPieceCache = 192;  // pieces of a CTA kept in shared memory; further ones are read from the table
 
 enum PlanBarrier : int {
-  kPbQFull = 0,      // +q    TMA -> MMA
-  kPbQEmpty = 2,     // +q    MMA -> TMA
-  kPbSFull = 4,      // +q    MMA -> softmax
-  kPbPReady = 6,     // +q    softmax (4 warps) -> MMA
-  kPbPvDone = 8,     // +q    MMA -> epilogue
-  kPbFin = 10,       // +q    softmax (4 warps) -> epilogue
-  kPbFinFree = 12,   // +q    epilogue (4 warps) -> softmax
-  kPbOFree = 14,     // +q    epilogue (4 warps) -> MMA
-  kPbPairFull = 16,  // +slot TMA -> MMA, warp 14
-  kPbPairEmpty = 18, // +slot MMA and warp 14 -> TMA
-  kPbTailClean = 20, // +slot warp 14 -> MMA: the rows of a V tile behind the last key are zero
-  kPbDrain = 22,
-  kNumPlanBarriers = 23
+  kPbQFull = 0,       // +lane * kQSlots + slot   TMA -> MMA
+  kPbQEmpty = 8,      // +lane * kQSlots + slot   MMA -> TMA
+  kPbSFull = 16,      // +lane  MMA -> softmax
+  kPbPReady = 18,     // +lane  softmax (4 warps) -> MMA
+  kPbPvDone = 20,     // +lane  MMA -> epilogue
+  kPbFin = 22,        // +lane  softmax (4 warps) -> epilogue
+  kPbFinFree = 24,    // +lane  epilogue (4 warps) -> softmax
+  kPbOFree = 26,      // +lane  epilogue (4 warps) -> MMA
+  kPbPairFull = 28,   // +slot  TMA -> MMA, warp 14
+  kPbPairEmpty = 30,  // +slot  MMA and warp 14 -> TMA
+  kPbTailClean = 32,  // +slot  warp 14 -> MMA: the rows of a V tile behind the last key are zero
+  kPbDrain = 34,
+  kNumPlanBarriers = 35
 };
 
 struct alignas(16) PlanAux {
@@ -134,16 +139,20 @@ __device__ __forceinline__ int piece_tail(const PlanPiece* pc) {
   return in_last < kBlockN ? in_last : 0;
 }
 
+// Pieces of one Q tile with few rows; on every lane they come after the larger ones.
+__device__ __forceinline__ bool is_small(const PlanParams& p, const PlanPiece* pc) {
+  return pc->tiles[1] == 0 && pc->n_tokens <= p.small_tokens;
+}
+
 // ---- TMA producer: K/V in pairs (V of one tile, K of the next), as in attn_fwd_ws_kernel -----------------
 __device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const PlanMaps& maps, uint32_t smem_q,
                                uint32_t smem_kv, uint32_t bar0, uint32_t lead, WaitCtx& w) {
   uint32_t slot = 0, empty_parity = 1;  // parity 1 passes on a fresh barrier
-  uint32_t q_empty_parity = 3;           // bit per lane
+  uint32_t q_empty_parity = 0xff;        // bit per Q slot
+  uint32_t small_loaded[2] = {0, 0};     // small pieces of each lane: the next one goes to slot small_loaded % 4
   uint32_t armed = 0, armed_parity = 0;  // for the early-exit path: "full" barriers armed, last parity of each
   bool ok = true;
   auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
-  const uint32_t q_bytes = uint32_t(p.tile_rows) * kHeadDim * 2;
-
   auto push_pair = [&](const PlanPiece* v_pc, int v_tile, const PlanPiece* k_pc, int k_tile, int site) -> bool {
     if (!w.wait_issue(bar(kPbPairEmpty + slot), empty_parity, site)) return false;
     const uint32_t full_parity = empty_parity ^ 1u;
@@ -169,18 +178,23 @@ __device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const Pl
     return true;
   };
 
-  // Q tile `tile` of a piece to a lane: a box of 64 columns x group heads x tile_tokens tokens lands as rows
+  // Q tile `tile` of a piece to a lane: a box of 64 columns x group heads x tokens lands as rows
   // token * group + head.
   auto load_q = [&](const PlanPiece* pc, int lane, int tile) -> bool {
-    if (!w.wait_issue(bar(kPbQEmpty + lane), (q_empty_parity >> lane) & 1u, 100 + lane)) return false;
-    q_empty_parity ^= 1u << lane;
-    armed |= 1u << (kPairSlotsP + lane);
-    armed_parity = (armed_parity & ~(1u << (kPairSlotsP + lane))) | (((q_empty_parity >> lane) & 1u) << (kPairSlotsP + lane));
-    const uint32_t full = bar(kPbQFull + lane), dst = smem_q + lane * kTileBytes;
+    const bool small = is_small(p, pc);
+    uint32_t n = 0;  // slot
+    if (small) n = (lane ? small_loaded[1]++ : small_loaded[0]++) % kQSlots;
+    const int s = lane * kQSlots + int(n);
+    if (!w.wait_issue(bar(kPbQEmpty + s), (q_empty_parity >> s) & 1u, 100 + s)) return false;
+    q_empty_parity ^= 1u << s;
+    armed |= 1u << (kPairSlotsP + s);
+    armed_parity = (armed_parity & ~(1u << (kPairSlotsP + s))) | (((q_empty_parity >> s) & 1u) << (kPairSlotsP + s));
+    const uint32_t full = bar(kPbQFull + s), dst = smem_q + lane * kTileBytes + n * (kQSlotRows * 128);
+    const CUtensorMap* tq = small ? &maps.q_small : &maps.q;
     const int token = pc->token + tile * p.tile_tokens;
-    mbar_arrive_expect_tx_lead(lead, full, q_bytes);
-    tma_load_4d_lead(lead, dst, &maps.q, 0, 0, pc->kv_head, token, full);
-    tma_load_4d_lead(lead, dst + kBoxBytes, &maps.q, 64, 0, pc->kv_head, token, full);
+    mbar_arrive_expect_tx_lead(lead, full, uint32_t((small ? p.small_tokens * p.group : p.tile_rows) * kHeadDim * 2));
+    tma_load_4d_lead(lead, dst, tq, 0, 0, pc->kv_head, token, full);
+    tma_load_4d_lead(lead, dst + kBoxBytes, tq, 64, 0, pc->kv_head, token, full);
     return true;
   };
 
@@ -200,31 +214,38 @@ __device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const Pl
     }
   }
   if (ok && ps.end > ps.pairs) {
+    // Q of a lane's pieces up to three ahead of piece `done`, or one ahead while pieces fill the whole buffer. The
+    // first small piece goes to slot 0 and so waits for the last large one; the others then find theirs free.
+    int next_q[2] = {ps.pairs, ps.lane1};
+    auto load_ahead = [&](int lane, int done) -> bool {
+      int n = lane ? next_q[1] : next_q[0];
+      const int end = lane ? ps.end : ps.lane1;
+      while (n < end && (n == done + 1 || (n < done + kQSlots && is_small(p, ps.at(done + 1))))) {
+        if (!load_q(ps.at(n), lane, 0)) return false;
+        ++n;
+      }
+      if (lane) next_q[1] = n; else next_q[0] = n;
+      return true;
+    };
     LaneWalk walk(ps);
-    const PlanPiece* pc = ps.at(ps.pairs);
-    ok = load_q(pc, 0, 0);
-    if (ok && ps.pairs == 0) ok = push_pair(nullptr, 0, pc, 0, 113);
-    if (ok && ps.lane1 < ps.end) {
-      pc = ps.at(ps.lane1);
-      ok = load_q(pc, 1, 0) && push_pair(nullptr, 0, pc, 0, 114);
-    }
+    ok = load_ahead(0, ps.pairs - 1);
+    if (ok && ps.pairs == 0) ok = push_pair(nullptr, 0, ps.at(0), 0, 113);
+    if (ok && ps.lane1 < ps.end) ok = load_ahead(1, ps.lane1 - 1) && push_pair(nullptr, 0, ps.at(ps.lane1), 0, 114);
     LaneWalk::Step st;
     while (ok && walk.take(ps, st)) {
-      pc = ps.at(st.piece);
+      const PlanPiece* pc = ps.at(st.piece);
       w.item = st.piece;
       w.tile = st.tile;
       if (!st.last) {
         ok = push_pair(pc, st.tile, pc, st.tile + 1, 115);
       } else {
-        const PlanPiece* following = walk.following(ps, st.lane);
-        ok = push_pair(pc, st.tile, following, 0, 116);
-        if (ok && following != nullptr) ok = load_q(following, st.lane, 0);
+        ok = push_pair(pc, st.tile, walk.following(ps, st.lane), 0, 116) && load_ahead(st.lane, st.piece);
       }
     }
   }
 
   if (!ok || w.aborted()) {
-    for (int s = 0; s < kPairSlotsP + kQTilesPerItem; ++s) {
+    for (int s = 0; s < kPairSlotsP + 2 * kQSlots; ++s) {
       if (!((armed >> s) & 1u)) continue;
       const uint32_t b = (s < kPairSlotsP) ? bar(kPbPairFull + s) : bar(kPbQFull + (s - kPairSlotsP));
       const uint64_t t0 = global_timer_ns();
@@ -291,7 +312,10 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
   auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
   uint32_t slot = 0, full_parity = 0;
   uint32_t tail_parity = 0;      // bit per slot
-  uint32_t q_full_parity = 0, p_parity = 0;  // bit per lane
+  uint32_t p_parity = 0;         // bit per lane
+  uint32_t q_full_parity = 0;    // bit per Q slot
+  uint32_t small_used[2] = {0, 0};
+  uint32_t q_slot[2] = {0, kQSlots};  // of the piece on each lane
   uint32_t o_free_parity = 3;    // passes on the fresh barrier: both accumulators start out free
   bool ok = true, k_ready = false;
 
@@ -301,14 +325,22 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
     if (slot == 0) full_parity ^= 1u;
     return true;  // the pair is the one in slot ^ 1
   };
-  // First scores of a piece on a lane, K in the pair waited for last.
-  auto first_scores = [&](int lane, int tiles) -> bool {
-    if (!w.wait_issue(bar(kPbQFull + lane), (q_full_parity >> lane) & 1u, 201 + lane)) return false;
-    q_full_parity ^= 1u << lane;
-    tc_fence_after_sync();
-    issue_qk(lead, tmem_base + lane * kBlockN, smem_q + lane * kTileBytes, smem_kv + (slot ^ 1u) * kPairBytesP + kTileBytes);
+  // Scores of a lane's piece with a K tile; after its last one the Q slot is free.
+  auto scores = [&](int lane, uint32_t k_smem, bool last) {
+    const uint32_t s = lane ? q_slot[1] : q_slot[0];
+    const uint32_t q = smem_q + lane * kTileBytes + (s % kQSlots) * (kQSlotRows * 128);
+    issue_qk(lead, tmem_base + lane * kBlockN, q, k_smem);
     umma_commit_lead(lead, bar(kPbSFull + lane));
-    if (tiles == 1) umma_commit_lead(lead, bar(kPbQEmpty + lane));
+    if (last) umma_commit_lead(lead, bar(kPbQEmpty + s));
+  };
+  // First scores of a piece on a lane, K in the pair waited for last.
+  auto first_scores = [&](int lane, const PlanPiece* pc, int tiles) -> bool {
+    const uint32_t s = lane * kQSlots + (is_small(p, pc) ? (lane ? small_used[1]++ : small_used[0]++) % kQSlots : 0u);
+    if (!w.wait_issue(bar(kPbQFull + s), (q_full_parity >> s) & 1u, 201 + lane)) return false;
+    q_full_parity ^= 1u << s;
+    if (lane) q_slot[1] = s; else q_slot[0] = s;
+    tc_fence_after_sync();
+    scores(lane, smem_kv + (slot ^ 1u) * kPairBytesP + kTileBytes, tiles == 1);
     return true;
   };
   // The V tile of the pair waited for last, if a piece's keys end inside it, once its other rows are zero.
@@ -345,7 +377,7 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
       k_ready = true;
     }
 #pragma unroll
-    for (int q = 0; q < kQTilesPerItem; ++q) ok = ok && first_scores(q, Tq[q]);
+    for (int q = 0; q < kQTilesPerItem; ++q) ok = ok && first_scores(q, pc, Tq[q]);
     if (!ok) break;
     // also covers the PV of the previous piece that read the V half of this pair
     umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
@@ -362,9 +394,7 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
         if (i < Tq[q]) {
           if (!(ok = weighted_sum(q, i, v_smem))) break;
           if (i + 1 < Tq[q]) {
-            issue_qk(lead, tmem_base + q * kBlockN, smem_q + q * kTileBytes, k_smem);
-            umma_commit_lead(lead, bar(kPbSFull + q));
-            if (i + 2 == Tq[q]) umma_commit_lead(lead, bar(kPbQEmpty + q));
+            scores(q, k_smem, i + 2 == Tq[q]);
           } else {
             umma_commit_lead(lead, bar(kPbPvDone + q));
           }
@@ -376,10 +406,10 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
   if (ok && ps.end > ps.pairs) {
     LaneWalk walk(ps);
     if (!k_ready) ok = wait_pair(203);
-    ok = ok && first_scores(0, walk.tiles[0]);
+    ok = ok && first_scores(0, ps.at(ps.pairs), walk.tiles[0]);
     if (ok) umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
     if (ok && ps.lane1 < ps.end) {
-      ok = wait_pair(204) && first_scores(1, walk.tiles[1]);
+      ok = wait_pair(204) && first_scores(1, ps.at(ps.lane1), walk.tiles[1]);
       if (ok) umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
     }
     LaneWalk::Step st;
@@ -392,14 +422,11 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
       if (st.last && piece_tail(ps.at(st.piece)) > 0 && !(ok = wait_tail())) break;
       if (!(ok = weighted_sum(lane, st.tile, v_smem))) break;
       if (!st.last) {
-        issue_qk(lead, tmem_base + lane * kBlockN, smem_q + lane * kTileBytes, v_smem + kTileBytes);
-        umma_commit_lead(lead, bar(kPbSFull + lane));
-        const int tiles = lane ? walk.tiles[1] : walk.tiles[0];
-        if (st.tile + 2 == tiles) umma_commit_lead(lead, bar(kPbQEmpty + lane));
+        scores(lane, v_smem + kTileBytes, st.tile + 2 == (lane ? walk.tiles[1] : walk.tiles[0]));
       } else {
         umma_commit_lead(lead, bar(kPbPvDone + lane));
         const PlanPiece* following = walk.following(ps, lane);
-        if (following != nullptr && !(ok = first_scores(lane, following->tiles[0]))) break;
+        if (following != nullptr && !(ok = first_scores(lane, following, following->tiles[0]))) break;
       }
       // nobody waits for the last pair to be handed back, and the CTA may be gone by then
       if (walk.more()) umma_commit_lead(lead, bar(kPbPairEmpty + (slot ^ 1u)));
@@ -658,8 +685,10 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
       w.raise(kDevSmemMisaligned, 3, 0);
     } else {
       for (int q = 0; q < kQTilesPerItem; ++q) {
-        mbar_init(bar0 + 8u * (kPbQFull + q), 1);
-        mbar_init(bar0 + 8u * (kPbQEmpty + q), 1);
+        for (int n = 0; n < kQSlots; ++n) {
+          mbar_init(bar0 + 8u * (kPbQFull + q * kQSlots + n), 1);
+          mbar_init(bar0 + 8u * (kPbQEmpty + q * kQSlots + n), 1);
+        }
         mbar_init(bar0 + 8u * (kPbSFull + q), 1);
         mbar_init(bar0 + 8u * (kPbPReady + q), 4);
         mbar_init(bar0 + 8u * (kPbPvDone + q), 1);

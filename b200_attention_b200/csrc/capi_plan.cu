@@ -156,6 +156,7 @@ int b200attn_forward_planned(const b200attn_planned_args* a) {
   p.group = group;
   p.tile_tokens = plan_tile_tokens(group);
   p.tile_rows = p.tile_tokens * group;
+  p.small_tokens = plan_small_tokens(group);
   const float scale = a->softmax_scale > 0.0f ? a->softmax_scale : 1.0f / std::sqrt(float(kHeadDim));
   p.scale_log2 = scale * 1.4426950408889634f;
   p.wait_limit_ms = g_wait_limit_ms.load(std::memory_order_relaxed);
@@ -167,6 +168,9 @@ int b200attn_forward_planned(const b200attn_planned_args* a) {
     kq.group = group;
     kq.box_tokens = p.tile_tokens;
     if ((rc = make_tensor_map(kq, &maps.q)) != 0) return rc;
+    maps.q_small = maps.q;
+    kq.box_tokens = p.small_tokens;
+    if (p.small_tokens > 0 && (rc = make_tensor_map(kq, &maps.q_small)) != 0) return rc;
     const b200attn_operand* src[4] = {&k, &v, &kp, &vp};
     CUtensorMap* dst[4] = {&maps.k, &maps.v, &maps.k_prefix, &maps.v_prefix};
     for (int i = 0; i < 4; ++i) {

@@ -22,12 +22,13 @@ constexpr int kTile = 128;
 // Costs in thousandths of the time of a K/V tile against two Q tiles (about 1.6 us). A piece of one Q tile runs on
 // one of a CTA's two lanes: alone it is bound by its chain of steps, beside another lane by what the two share.
 constexpr int64_t kTilePair = 1000;
-constexpr int64_t kPairStart = 1500;    // Q load, first scores, last PV, stores
-constexpr int64_t kTileShared = 600;    // tensor pipe and memory, per tile of a lane
+constexpr int64_t kPairStart = 1800;    // Q load, first scores, last PV, stores
+constexpr int64_t kTileShared = 900;    // memory and tensor pipe, per tile of a lane
 constexpr int64_t kSharedStart = 500;
-constexpr int64_t kTileChain = 850;     // scores, softmax, PV of one tile after the other
-constexpr int64_t kChainStart = 1200;
-constexpr int64_t kJoin = 2500;         // the second kernel, once
+constexpr int64_t kTileChain = 950;     // scores, softmax, PV of one tile after the other
+constexpr int64_t kChainStart = 1500;
+constexpr int64_t kJoin = 2200;         // the second kernel, once,
+constexpr int64_t kJoinRows = 17;       // and per row of partial results, divided by this: written, then read, by all CTAs
 
 struct Item {
   int32_t token, n_tokens, kv_row, n_keys, tiles0, tiles1, diag, kv_head, source;
@@ -36,13 +37,14 @@ struct Item {
 };
 
 struct Cost {
-  bool pair;
+  int32_t kind;    // 2: two Q tiles, 1: one, 0: one with few rows; in this order on every CTA
   int64_t shared;  // of the CTA's time
   int64_t chain;   // of a lane's time, for one Q tile
 };
-Cost cost_of(const PlanPiece& p) {
-  if (p.tiles[1] > 0) return {true, kPairStart + p.tiles[1] * kTilePair, 0};
-  return {false, kSharedStart + p.tiles[0] * kTileShared, kChainStart + p.tiles[0] * kTileChain};
+Cost cost_of(const PlanPiece& p, int32_t small_tokens) {
+  if (p.tiles[1] > 0) return {2, kPairStart + p.tiles[1] * kTilePair, 0};
+  return {p.n_tokens <= small_tokens ? 0 : 1, kSharedStart + p.tiles[0] * kTileShared,
+          kChainStart + p.tiles[0] * kTileChain};
 }
 
 // Piece `c` of an item cut every `len` tiles.
@@ -93,7 +95,7 @@ struct Dealer {
     free.pop();
     Cta& t = cta[size_t(at)];
     int32_t lane = 0;
-    if (c.pair) {
+    if (c.kind == 2) {
       t.pairs += c.shared;
     } else {
       lane = t.lane[1] < t.lane[0] ? 1 : 0;
@@ -112,7 +114,7 @@ struct Dealer {
 };
 
 bool longer(const Cost& a, const Cost& b) {
-  if (a.pair != b.pair) return a.pair;  // pieces of two Q tiles come first on every CTA
+  if (a.kind != b.kind) return a.kind > b.kind;
   return a.shared > b.shared;
 }
 
@@ -128,7 +130,7 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   if (in.len_prefix < 0 || in.len_prefix >= (1 << 30)) return "len_prefix must be 0 .. 2^30 - 1";
 
   const int32_t tile_tokens = plan_tile_tokens(group);
-  const int32_t block = 2 * tile_tokens;
+  const int32_t block = 2 * tile_tokens, small_tokens = plan_small_tokens(group);
   std::vector<int64_t> first_token(size_t(in.sequences) + 1, 0), first_key(size_t(in.sequences), 0);
   int64_t at = 0;
   plan->rows_kv = 0;
@@ -230,15 +232,18 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
     for (const int32_t len : lens) {
       costs.clear();
       bool any_cut = has_prefix;
+      int64_t rows = 0;
       for (const Item& it : items) {
         const int32_t n = cuts_of(it, len), l = even_len(it, len);
         any_cut = any_cut || n > 1;
-        for (int32_t c = 0; c < n; ++c) costs.push_back(cost_of(cut_piece(it, c * l, std::min(l, it.longest() - c * l))));
+        for (int32_t c = 0; c < n; ++c)
+          costs.push_back(cost_of(cut_piece(it, c * l, std::min(l, it.longest() - c * l)), small_tokens));
+        if (n > 1 || has_prefix) rows += int64_t(n) * it.n_tokens * group;
       }
       std::sort(costs.begin(), costs.end(), longer);
       Dealer dealer(in.sm_count);
       for (const Cost& c : costs) dealer.deal(c);
-      const int64_t end = dealer.end() + (any_cut ? kJoin : 0);
+      const int64_t end = dealer.end() + (any_cut ? kJoin + rows / kJoinRows : 0);
       if (best < 0 || end < best) {
         best = end;
         best_len = len;
@@ -269,7 +274,7 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
         slots += int64_t(it.n_tokens) * group;
         if (slots >= (int64_t(1) << 31) - 512) return "too many partial rows";
       }
-      p.cost = cost_of(p.p);
+      p.cost = cost_of(p.p, small_tokens);
       p.head_group = by_groups ? it.kv_head / 16 : 0;
       pieces.push_back(p);
     }
@@ -330,7 +335,7 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   for (size_t i = 0; i < order.size(); ++i) order[i] = int32_t(i);
   std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) {
     const Piece &x = pieces[size_t(a)], &y = pieces[size_t(b)];
-    if (x.cost.pair == y.cost.pair && x.head_group != y.head_group) return x.head_group < y.head_group;
+    if (x.cost.kind == y.cost.kind && x.head_group != y.head_group) return x.head_group < y.head_group;
     return longer(x.cost, y.cost);
   });
   std::vector<std::vector<int32_t>> dealt(size_t(in.sm_count) * 3);  // pairs, lane 0, lane 1 of each CTA
@@ -338,7 +343,7 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   for (const int32_t i : order) {
     const Cost& c = pieces[size_t(i)].cost;
     const Dealer::Place at = dealer.deal(c);
-    dealt[size_t(at.cta) * 3 + size_t(c.pair ? 0 : 1 + at.lane)].push_back(i);
+    dealt[size_t(at.cta) * 3 + size_t(c.kind == 2 ? 0 : 1 + at.lane)].push_back(i);
   }
   plan->grid = 0;
   for (int32_t c = 0; c < in.sm_count; ++c)

@@ -72,5 +72,6 @@ struct Plan {
 std::string plan_build(const PlanInput& in, Plan* plan);
 
 inline int32_t plan_tile_tokens(int32_t group) { return 128 / group; }
+inline int32_t plan_small_tokens(int32_t group) { return 32 / group; }
 
 }  // namespace b200attn

@@ -6,9 +6,10 @@
 
 namespace b200attn {
 
-// q: (head_dim, head of the group, K/V head, token); the others: (head_dim, row, K/V head, 1)
+// q, q_small: (head_dim, head of the group, K/V head, token), boxes of tile_tokens and small_tokens tokens; the others:
+// (head_dim, row, K/V head, 1)
 struct PlanMaps {
-  CUtensorMap q, k, v, k_prefix, v_prefix;
+  CUtensorMap q, q_small, k, v, k_prefix, v_prefix;
 };
 
 struct PlanParams {
@@ -21,6 +22,7 @@ struct PlanParams {
   int32_t group;        // query heads per K/V head
   int32_t tile_tokens;  // floor(128 / group)
   int32_t tile_rows;    // tile_tokens * group
+  int32_t small_tokens; // floor(32 / group): a piece of one Q tile with at most these is a small one; may be 0
   float scale_log2;
   int32_t* status;
   uint32_t wait_limit_ms;

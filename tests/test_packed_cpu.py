@@ -33,6 +33,9 @@ def expand(lens_q, lens_kv, heads, heads_kv, *, causal, starts=None, prefix=0, s
     for pairs, lane0, lane1, end in ctas.tolist():
         assert both[pairs:lane0].all() and not both[lane0:end].any()
         assert lane1 > lane0 or end == lane1, "lane 1 has work, lane 0 none"
+        for a, b in ((lane0, lane1), (lane1, end)):  # pieces that fill the lane's Q buffer come before those that share it
+            small = pieces[a:b, 1] <= 32 // group
+            assert (small[:-1] <= small[1:]).all()
     runs, slot_owner = {}, {}
     for token, n, row, keys, tiles0, tiles1, diag, head, source, slot in pieces[:, :10].tolist():
         assert 1 <= n <= 2 * per_tile and keys > 0 and tiles0 >= 1
@@ -122,7 +125,8 @@ def test_random_schedules(native_built):
 
 
 def test_work_is_spread_evenly(native_built):
-    """Tiles of the busiest CTA against the mean."""
+    """Pieces go to the CTA that is free first, so when a CTA took its last one no other had less: its load is at most
+    the mean load and one piece more. Counted in K/V tiles; a piece's start counts as up to 2."""
     for lens_q, lens_kv, heads, heads_kv in [([16384], [16384], 16, 16), ([1], [65536], 32, 8),
                                              ([1] * 64, [100 + (i * 4463) % 11901 for i in range(64)], 32, 8),
                                              ([2500] * 5, [2500] * 5, 8, 2)]:
@@ -130,8 +134,11 @@ def test_work_is_spread_evenly(native_built):
         t = s.table.numpy()
         pieces = t[PIECE_AT:PIECE_AT + 12 * s.info.pieces].reshape(-1, 12)
         ctas = t[CTA_AT:PIECE_AT].reshape(160, 4)
-        tiles = [pieces[a:b, 4:6].max(1).sum() for a, b in ctas[:148, [0, 3]]]
-        assert max(tiles) <= 1.15 * np.mean(tiles) + 3
+        tiles = pieces[:, 4:6].max(1)
+        load = [tiles[a:b].sum() for a, b in ctas[:148, [0, 3]]]
+        assert max(load) <= np.mean(load) + 2 * s.info.pieces / 148 + tiles.max() + 2
+    one = packed.Schedule([1], [65536], heads=32, heads_kv=8)
+    assert one.info.grid == 148  # a single token's keys are cut so that every CTA has some
 
 
 @pytest.mark.parametrize("kw, error", [
