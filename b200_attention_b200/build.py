@@ -27,7 +27,7 @@ ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CORE_SOURCES = [CSRC / "attn_fwd_sm100.cu", CSRC / "capi.cu", CSRC / "noalloc.cu", CSRC / "attn_plan_sm100.cu",
                 CSRC / "rotary_sm100.cu", CSRC / "capi_plan.cu", CSRC / "plan.cpp"]
 CORE_HEADERS = [CSRC / "attn_device_sm100.cuh", CSRC / "attn_kernels.cuh", CSRC / "ptx_sm100.cuh", CSRC / "host_common.cuh",
-                CSRC / "plan.h", CSRC / "plan_kernels.cuh", CSRC / "rotary_kernels.cuh",
+                CSRC / "plan.h", CSRC / "plan_kernels.cuh", CSRC / "launch_overlap.cuh", CSRC / "rotary_kernels.cuh",
                 INCLUDE / "b200_attention.h"]
 
 

@@ -26,6 +26,7 @@
 // that nobody looks at.)
 
 #include "attn_device_sm100.cuh"
+#include "launch_overlap.cuh"
 #include "plan_kernels.cuh"
 
 namespace b200attn {
@@ -145,15 +146,23 @@ __device__ __forceinline__ bool is_small(const PlanParams& p, const PlanPiece* p
 }
 
 // ---- TMA producer: K/V in pairs (V of one tile, K of the next), as in attn_fwd_ws_kernel -----------------
-__device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const PlanMaps& maps, uint32_t smem_q,
-                               uint32_t smem_kv, uint32_t bar0, uint32_t lead, WaitCtx& w) {
-  uint32_t slot = 0, empty_parity = 1;  // parity 1 passes on a fresh barrier
+struct Loader {
+  const PlanParams& p;
+  const PlanMaps& maps;
+  uint32_t smem_q, smem_kv, bar0, lead;
+  uint32_t slot = 0, empty_parity = 1;   // parity 1 passes on a fresh barrier
   uint32_t q_empty_parity = 0xff;        // bit per Q slot
   uint32_t small_loaded[2] = {0, 0};     // small pieces of each lane: the next one goes to slot small_loaded % 4
   uint32_t armed = 0, armed_parity = 0;  // for the early-exit path: "full" barriers armed, last parity of each
-  bool ok = true;
-  auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
-  auto push_pair = [&](const PlanPiece* v_pc, int v_tile, const PlanPiece* k_pc, int k_tile, int site) -> bool {
+
+  __device__ __forceinline__ Loader(const PlanParams& p_, const PlanMaps& m_, uint32_t q_, uint32_t kv_, uint32_t b_,
+                                    uint32_t lead_)
+      : p(p_), maps(m_), smem_q(q_), smem_kv(kv_), bar0(b_), lead(lead_) {}
+  __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8u * uint32_t(i); }
+
+  // V tile of one piece (or none) and K tile of one (or none) to the next slot of the ring.
+  __device__ __forceinline__ bool push_pair(const PlanPiece* v_pc, int v_tile, const PlanPiece* k_pc, int k_tile, int site,
+                                            const WaitCtx& w) {
     if (!w.wait_issue(bar(kPbPairEmpty + slot), empty_parity, site)) return false;
     const uint32_t full_parity = empty_parity ^ 1u;
     armed |= 1u << slot;
@@ -176,11 +185,11 @@ __device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const Pl
     slot ^= 1u;
     if (slot == 0) empty_parity ^= 1u;
     return true;
-  };
+  }
 
   // Q tile `tile` of a piece to a lane: a box of 64 columns x group heads x tokens lands as rows
   // token * group + head.
-  auto load_q = [&](const PlanPiece* pc, int lane, int tile) -> bool {
+  __device__ __forceinline__ bool load_q(const PlanPiece* pc, int lane, int tile, const WaitCtx& w) {
     const bool small = is_small(p, pc);
     uint32_t n = 0;  // slot
     if (small) n = (lane ? small_loaded[1]++ : small_loaded[0]++) % kQSlots;
@@ -196,65 +205,73 @@ __device__ void plan_load_role(const PlanParams& p, const PlanAux* aux, const Pl
     tma_load_4d_lead(lead, dst, tq, 0, 0, pc->kv_head, token, full);
     tma_load_4d_lead(lead, dst + kBoxBytes, tq, 64, 0, pc->kv_head, token, full);
     return true;
-  };
-
-  const Pieces ps(p, aux);
-  if (ps.pairs > 0) ok = push_pair(nullptr, 0, ps.at(0), 0, 110);  // the first K tile travels alone
-  for (int n = 0; ok && n < ps.pairs; ++n) {
-    const PlanPiece* pc = ps.at(n);
-    const int T = pc->tiles[1];
-    w.item = n;
-    w.tile = 0;
-    for (int q = 0; ok && q < kQTilesPerItem; ++q) ok = load_q(pc, q, q);
-    for (int i = 0; ok && i < T; ++i) {
-      w.tile = i;
-      // the last V with the first K of the CTA's next piece, if any (it is lane 0's, if the pairs end here)
-      const bool last = i + 1 == T;
-      ok = push_pair(pc, i, !last ? pc : n + 1 < ps.end ? ps.at(n + 1) : nullptr, last ? 0 : i + 1, 111);
-    }
-  }
-  if (ok && ps.end > ps.pairs) {
-    // Q of a lane's pieces up to three ahead of piece `done`, or one ahead while pieces fill the whole buffer. The
-    // first small piece goes to slot 0 and so waits for the last large one; the others then find theirs free.
-    int next_q[2] = {ps.pairs, ps.lane1};
-    auto load_ahead = [&](int lane, int done) -> bool {
-      int n = lane ? next_q[1] : next_q[0];
-      const int end = lane ? ps.end : ps.lane1;
-      while (n < end && (n == done + 1 || (n < done + kQSlots && is_small(p, ps.at(done + 1))))) {
-        if (!load_q(ps.at(n), lane, 0)) return false;
-        ++n;
-      }
-      if (lane) next_q[1] = n; else next_q[0] = n;
-      return true;
-    };
-    LaneWalk walk(ps);
-    ok = load_ahead(0, ps.pairs - 1);
-    if (ok && ps.pairs == 0) ok = push_pair(nullptr, 0, ps.at(0), 0, 113);
-    if (ok && ps.lane1 < ps.end) ok = load_ahead(1, ps.lane1 - 1) && push_pair(nullptr, 0, ps.at(ps.lane1), 0, 114);
-    LaneWalk::Step st;
-    while (ok && walk.take(ps, st)) {
-      const PlanPiece* pc = ps.at(st.piece);
-      w.item = st.piece;
-      w.tile = st.tile;
-      if (!st.last) {
-        ok = push_pair(pc, st.tile, pc, st.tile + 1, 115);
-      } else {
-        ok = push_pair(pc, st.tile, walk.following(ps, st.lane), 0, 116) && load_ahead(st.lane, st.piece);
-      }
-    }
   }
 
-  if (!ok || w.aborted()) {
-    for (int s = 0; s < kPairSlotsP + 2 * kQSlots; ++s) {
-      if (!((armed >> s) & 1u)) continue;
-      const uint32_t b = (s < kPairSlotsP) ? bar(kPbPairFull + s) : bar(kPbQFull + (s - kPairSlotsP));
-      const uint64_t t0 = global_timer_ns();
-      while (!mbar_try_wait(b, (armed_parity >> s) & 1u, 1000)) {
-        if (global_timer_ns() - t0 > w.limit_ns) break;
+  // Q and the first K tile (which travels alone) of the CTA's first piece; on barriers that nobody has used yet.
+  __device__ __forceinline__ void begin(const PlanPiece* pc, const WaitCtx& w) {
+    load_q(pc, 0, 0, w);
+    push_pair(nullptr, 0, pc, 0, 110, w);
+    if (pc->tiles[1] > 0) load_q(pc, 1, 1, w);
+  }
+
+  __device__ void run(const PlanAux* aux, WaitCtx& w) {
+    const Pieces ps(p, aux);
+    bool ok = true;
+    for (int n = 0; ok && n < ps.pairs; ++n) {
+      const PlanPiece* pc = ps.at(n);
+      const int T = pc->tiles[1];
+      w.item = n;
+      w.tile = 0;
+      for (int q = 0; ok && n > 0 && q < kQTilesPerItem; ++q) ok = load_q(pc, q, q, w);
+      for (int i = 0; ok && i < T; ++i) {
+        w.tile = i;
+        // the last V with the first K of the CTA's next piece, if any (it is lane 0's, if the pairs end here)
+        const bool last = i + 1 == T;
+        ok = push_pair(pc, i, !last ? pc : n + 1 < ps.end ? ps.at(n + 1) : nullptr, last ? 0 : i + 1, 111, w);
+      }
+    }
+    if (ok && ps.end > ps.pairs) {
+      // Q of a lane's pieces up to three ahead of piece `done`, or one ahead while pieces fill the whole buffer. The
+      // first small piece goes to slot 0 and so waits for the last large one; the others then find theirs free.
+      int next_q[2] = {ps.pairs, ps.lane1};
+      auto load_ahead = [&](int lane, int done, int most) -> bool {
+        int n = lane ? next_q[1] : next_q[0];
+        const int end = min(lane ? ps.end : ps.lane1, n + most);
+        while (n < end && (n == done + 1 || (n < done + kQSlots && is_small(p, ps.at(done + 1))))) {
+          if (!load_q(ps.at(n), lane, 0, w)) return false;
+          ++n;
+        }
+        if (lane) next_q[1] = n; else next_q[0] = n;
+        return true;
+      };
+      LaneWalk walk(ps);
+      if (ps.pairs == 0) next_q[0] = 1; else ok = load_ahead(0, ps.pairs - 1, 1);
+      if (ok && ps.lane1 < ps.end)
+        ok = load_ahead(1, ps.lane1 - 1, 1) && push_pair(nullptr, 0, ps.at(ps.lane1), 0, 114, w);
+      LaneWalk::Step st;
+      while (ok && walk.take(ps, st)) {
+        const PlanPiece* pc = ps.at(st.piece);
+        w.item = st.piece;
+        w.tile = st.tile;
+        const PlanPiece* k_pc = st.last ? walk.following(ps, st.lane) : pc;
+        ok = push_pair(pc, st.tile, k_pc, st.last ? 0 : st.tile + 1, 115, w);
+        // a piece's first step fetches ahead; so does its last, in case the next piece had to wait for the buffer
+        if (ok && (st.last || st.tile == 0)) ok = load_ahead(st.lane, st.last ? st.piece : st.piece - 1, kQSlots);
+      }
+    }
+
+    if (!ok || w.aborted()) {
+      for (int s = 0; s < kPairSlotsP + 2 * kQSlots; ++s) {
+        if (!((armed >> s) & 1u)) continue;
+        const uint32_t b = (s < kPairSlotsP) ? bar(kPbPairFull + s) : bar(kPbQFull + (s - kPairSlotsP));
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(b, (armed_parity >> s) & 1u, 1000)) {
+          if (global_timer_ns() - t0 > w.limit_ns) break;
+        }
       }
     }
   }
-}
+};
 
 // ---- V tails ------------------------------------------------------------------------------------------
 // Sees every pair (it takes part in handing pairs back, so it can never miss a phase). Where the V tile holds
@@ -444,9 +461,12 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
 }
 
 // ---- softmax: one row per thread -------------------------------------------------------------------------
-// As in attn_fwd_ws_kernel (speculative against the row's reference maximum, exact where the tile's sum says
-// that it has to move), plus rows that see no key of a tile, or of the whole piece: their m stays -inf, which
-// sends the row down the exact path, where it is subtracted as 0 so that every probability is 2^-inf = 0.
+// As in attn_fwd_ws_kernel: speculative against the row's reference maximum, exact where the tile's sum says that it
+// has to move. Two differences. The first tile speculates too, on a reference of 0: any reference within 2^32 of the
+// true one serves, so the tile stands if its sum lies between 2^-32 and 2^32, and the pass over it for its maximum is
+// only needed for larger scores (it costs a third of a tile's time, which a piece of a few tiles feels). And rows that
+// see no key of a tile, or of the whole piece: their m becomes -inf, which sends them down the exact path, where it is
+// subtracted as 0 so that every probability is 2^-inf = 0.
 __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t bar0, uint32_t tmem_base, int q,
                                   int warp_in_group, int lane, WaitCtx& w) {
   auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
@@ -480,8 +500,8 @@ __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t ba
     w.tile = 0;
     if (!w.wait_warp(bar(kPbFinFree + q), fin_free_parity, 310 + q)) return;
     fin_free_parity ^= 1u;
-    float m = kNegInf;  // reference maximum, log2 units
-    float l = 0.0f;     // running sum of 2^(s - m)
+    float m = 0.0f;  // reference maximum, log2 units
+    float l = 0.0f;  // running sum of 2^(s - m)
     for (int i = 0; i < T; ++i) {
       w.tile = i;
       if (!w.wait_warp(bar(kPbSFull + q), s_parity, 300 + q)) return;
@@ -496,33 +516,31 @@ __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t ba
         tmem_ld32(s_tmem + 96, s[3]);
         const bool tail = i * kBlockN + kBlockN - 1 > tile_limit;  // uniform across the warp
         const int valid = row_limit - i * kBlockN + 1;             // keys of this tile that the row sees
-        if (tail || i == 0) tmem_wait_ld();
-        if (tail) mask_tail(s, valid);
+        if (tail) {
+          tmem_wait_ld();
+          mask_tail(s, valid);
+        }
 
         uint32_t packed[4][16];
         f2 sum_a = f2_splat(0.0f), sum_b = f2_splat(0.0f);
-        float tile_sum = 0.0f;
-        bool exact = (i == 0);
-        if (!exact) {
+        {
           const f2 neg_m2 = f2_splat(-m);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             exp_chunk(s[c], scale2, neg_m2, packed[c], sum_a, sum_b);
             if (c == 0) tmem_wait_ld();
           }
-          tile_sum = f2_hsum(sum_a, sum_b);
-          // written so that a NaN sum also lands on the exact path
-          exact = __any_sync(0xffffffffu, row_live && !(tile_sum < sum_limit));
         }
-        if (__builtin_expect(exact, 0)) {
-          if (i > 0) {
+        float tile_sum = f2_hsum(sum_a, sum_b);
+        // written so that a NaN sum also lands on the exact path
+        const bool stands = tile_sum < sum_limit && (i > 0 || tile_sum > 1.0f / sum_limit);
+        if (__builtin_expect(__any_sync(0xffffffffu, row_live && !stands), 0)) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, s[c]);
-            tmem_wait_ld();
-            if (tail) mask_tail(s, valid);
-          }
+          for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, s[c]);
+          tmem_wait_ld();
+          if (tail) mask_tail(s, valid);
           const float tile_max = row_max(s) * scale_log2;
-          const float m_new = fmaxf(m, tile_max);
+          const float m_new = i == 0 ? tile_max : fmaxf(m, tile_max);
           if (i > 0) {
             const float f = m_new == kNegInf ? 1.0f : ex2_approx(m - m_new);
             l *= f;
@@ -607,24 +625,28 @@ __device__ void plan_epilogue_role(const PlanParams& p, const PlanAux* aux, uint
       constexpr int kChunk = 16;
       if (any_live) {
 #pragma unroll 1
-        for (int c = 0; c < kHeadDim / kChunk; ++c) {
-          uint32_t acc[kChunk];
-          tmem_ld16(o_row + c * kChunk, acc);
+        for (int c = 0; c < kHeadDim / kChunk; c += 2) {
+          uint32_t acc[2][kChunk];
+          tmem_ld16(o_row + c * kChunk, acc[0]);
+          tmem_ld16(o_row + (c + 1) * kChunk, acc[1]);
           tmem_wait_ld();
           if (!live) continue;
-          float v[kChunk];
 #pragma unroll
-          for (int j = 0; j < kChunk; ++j) v[j] = seen ? __uint_as_float(acc[j]) * weight : 0.0f;
-          if (slot_row >= 0) {
-            float4* dst = reinterpret_cast<float4*>(part + c * kChunk);
+          for (int u = 0; u < 2; ++u) {
+            float v[kChunk];
 #pragma unroll
-            for (int j = 0; j < kChunk / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          } else {
-            uint4* dst = reinterpret_cast<uint4*>(out + c * kChunk);
+            for (int j = 0; j < kChunk; ++j) v[j] = seen ? __uint_as_float(acc[u][j]) * weight : 0.0f;
+            if (slot_row >= 0) {
+              float4* dst = reinterpret_cast<float4*>(part + (c + u) * kChunk);
 #pragma unroll
-            for (int j = 0; j < kChunk / 8; ++j)
-              dst[j] = make_uint4(pack_bf16x2(v[8 * j + 0], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                                  pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+              for (int j = 0; j < kChunk / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(out + (c + u) * kChunk);
+#pragma unroll
+              for (int j = 0; j < kChunk / 8; ++j)
+                dst[j] = make_uint4(pack_bf16x2(v[8 * j + 0], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                                    pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+            }
           }
         }
       }
@@ -671,19 +693,35 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
   w.item = -1;
   w.tile = -1;
 
+  // The next kernel of the stream may be brought up from here on; it waits for the end of this one before it touches
+  // anything that this one writes, as this one does below (also where it has nothing to do, so that whoever waits for
+  // this kernel has waited for the ones before it).
+  launch_dependents();
   const bool misaligned = (smem_q & 1023u) != 0;  // uniform across the CTA
   const int4 first = reinterpret_cast<const int4*>(p.table + kPlanCtaAt)[blockIdx.x];
   const int piece0 = first.x, piece1 = first.w;
-  if (piece0 >= piece1) return;  // uniform across the CTA: a table with fewer CTAs than the grid
-  if (threadIdx.x == 0) {
-    aux->abort_flag = 0;
-    aux->first[0] = first.x;
-    aux->first[1] = first.y;
-    aux->first[2] = first.z;
-    aux->first[3] = first.w;
-    if (misaligned) {
+  if (misaligned || piece0 >= piece1) {  // uniform across the CTA; the latter: a table with fewer CTAs than the grid
+    if (threadIdx.x == 0 && misaligned) {
+      aux->abort_flag = 0;
       w.raise(kDevSmemMisaligned, 3, 0);
-    } else {
+    }
+    wait_for_previous();
+    return;
+  }
+  const uint32_t lead = (lane == 0) ? 1u : 0u;
+  Loader loader(p, maps, smem_q, smem_kv, bar0, lead);
+  if (warp == 13) {
+    if (lane < 6) tma_prefetch_desc(&maps.q + lane);
+    const int4* src = reinterpret_cast<const int4*>(p.table + kPlanPieceAt) + size_t(piece0) * 3;
+    alignas(16) PlanPiece piece;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) reinterpret_cast<int4*>(&piece)[j] = src[j];
+    if (lane == 0) {
+      aux->abort_flag = 0;
+      aux->first[0] = first.x;
+      aux->first[1] = first.y;
+      aux->first[2] = first.z;
+      aux->first[3] = first.w;
       for (int q = 0; q < kQTilesPerItem; ++q) {
         for (int n = 0; n < kQSlots; ++n) {
           mbar_init(bar0 + 8u * (kPbQFull + q * kQSlots + n), 1);
@@ -705,13 +743,16 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
       mbar_init_fence();
       fence_proxy_async_smem();
     }
-  }
-  if (misaligned) return;
-  {
+    __syncwarp();
+    // The whole CTA waits here (at the barrier below), before any of its bounded waits begin.
+    wait_for_previous();
+    loader.begin(&piece, w);  // under way while the rest of the CTA sets itself up
+  } else {
     const int4* src = reinterpret_cast<const int4*>(p.table + kPlanPieceAt) + size_t(piece0) * 3;
     int4* dst = reinterpret_cast<int4*>(aux->cache);
     const int words = min(piece1 - piece0, kPieceCache) * 3;
-    for (int j = threadIdx.x; j < words; j += kPlanThreads) dst[j] = src[j];
+    if (threadIdx.x < 384)  // warps 0 to 11
+      for (int j = threadIdx.x; j < words; j += 384) dst[j] = src[j];
   }
   if (warp == 12) {
     tmem_alloc(smem_u32(&aux->tmem_base), 512);
@@ -730,11 +771,10 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
     plan_epilogue_role(p, aux, bar0, tmem_base, warp & 3, lane, w);
   } else {
     reg_shrink<kPlanRegsOther>();
-    const uint32_t lead = (lane == 0) ? 1u : 0u;
     if (warp == 12) {
       plan_mma_role(p, aux, smem_q, smem_kv, bar0, tmem_base, lead, w);
     } else if (warp == 13) {
-      plan_load_role(p, aux, maps, smem_q, smem_kv, bar0, lead, w);
+      loader.run(aux, w);
     } else if (warp == 14) {
       plan_tail_role(p, aux, kv, bar0, lane, w);
     }
@@ -750,75 +790,151 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
 }
 
 // ---- join ---------------------------------------------------------------------------------------------------
-// A block per unit (at most 32 rows, or one token), a warp per row: the lanes find the row's total LSE over its
-// parts, then the warp adds the weighted partial rows, four in flight, lane l holding columns 4l .. 4l + 3.
-// Rows without a part get O = 0 and LSE = -inf. Reads 512 B per part and row: at 64 requests x 32 heads with
-// ten parts 10.5 MB, which the partials' stay in L2 makes a matter of latency.
+// A block per unit (at most 32 rows, or one token), lane l of a warp holding columns 4l .. 4l + 3 of a row. Parts are
+// taken with a running reference and sum, so that LSEs and partial rows are on their way together and nothing waits for
+// a pass over the LSEs first. A warp has the parts of two rows in flight where there are at most two, else four parts
+// of one row, and a unit of fewer than eight rows spreads the parts of a row over several warps. 64 registers: the
+// blocks of 512 units are then resident together (eight parts in flight took 79 registers and twice as long there).
+// Rows without a part, and rows whose parts saw no key, get O = 0 and LSE = -inf. Bound by latency for few rows
+// (64 tokens x 32 heads, 9 parts: 5.1 us), else by reading 516 bytes per part and row (82 thousand: 12.3 us).
 constexpr int kJoinWarps = 8;
-__global__ void __launch_bounds__(kJoinWarps * 32)
+
+struct JoinState {
+  float m, sum;
+  float4 acc;
+  __device__ __forceinline__ void clear() {
+    m = kNegInf;
+    sum = 0.0f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  __device__ __forceinline__ void rebase(float top) {  // top >= m
+    const float f = m == top ? 1.0f : expf(m - top);
+    m = top;
+    sum *= f;
+    acc.x *= f;
+    acc.y *= f;
+    acc.z *= f;
+    acc.w *= f;
+  }
+  __device__ __forceinline__ void add(float weight, const float4& a, float s) {
+    sum = fmaf(weight, s, sum);
+    acc.x = fmaf(a.x, weight, acc.x);
+    acc.y = fmaf(a.y, weight, acc.y);
+    acc.z = fmaf(a.z, weight, acc.z);
+    acc.w = fmaf(a.w, weight, acc.w);
+  }
+};
+
+// Weight of something with LSE or reference `of` against `top` >= of: 0 where it saw no key.
+__device__ __forceinline__ float join_weight(float of, float top) { return expf(of - (top == kNegInf ? 0.0f : top)); }
+
+__device__ __forceinline__ void join_store(const PlanParams& p, const PlanUnit& un, int r, int lane, const JoinState& s) {
+  const int token = r / p.group;
+  const int head = un.kv_head * p.group + (r - token * p.group);
+  const int64_t row = int64_t(un.token) + token;
+  const bool seen = s.sum != 0.0f;  // a NaN sum counts as seen
+  const float inv = seen ? 1.0f / s.sum : 0.0f;
+  uint2 out;
+  out.x = pack_bf16x2(s.acc.x * inv, s.acc.y * inv);
+  out.y = pack_bf16x2(s.acc.z * inv, s.acc.w * inv);
+  *reinterpret_cast<uint2*>(p.o + row * p.o_stride_t + int64_t(head) * p.o_stride_h + lane * 4) = out;
+  if (p.lse != nullptr && lane == 0)
+    p.lse[int64_t(head) * p.lse_stride_h + row] = seen ? s.m + logf(s.sum) : kNegInf;
+}
+
+// Parts k0, k0 + step, .. of rows r0 .. r0 + kRows - 1 (those below `rows`), kParts of them at a time.
+template <int kRows, int kParts>
+__device__ __forceinline__ void join_rows(const PlanParams& p, const int32_t* parts, int n_parts, int k0, int step, int r0,
+                                          int rows, int lane, JoinState (&s)[kRows]) {
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) s[i].clear();
+  for (int k = k0; k < n_parts; k += step * kParts) {
+    float lse[kRows][kParts];
+    float4 a[kRows][kParts];
+#pragma unroll
+    for (int j = 0; j < kParts; ++j) {
+      const bool there = k + j * step < n_parts;
+      const int at = (there ? parts[k + j * step] : 0) + r0;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        lse[i][j] = kNegInf;
+        a[i][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (there && r0 + i < rows) {
+          lse[i][j] = __ldcg(p.part_lse + at + i);
+          a[i][j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + int64_t(at + i) * kHeadDim) + lane);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      float top = s[i].m;
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) top = fmaxf(top, lse[i][j]);
+      s[i].rebase(top);
+#pragma unroll
+      for (int j = 0; j < kParts; ++j) s[i].add(join_weight(lse[i][j], top), a[i][j], 1.0f);
+    }
+  }
+}
+
+template <int kRows, int kParts>
+__device__ __forceinline__ void join_unit(const PlanParams& p, const PlanUnit& un, const int32_t* parts, int rows, int warp,
+                                          int lane) {
+  for (int r0 = warp * kRows; r0 < rows; r0 += kJoinWarps * kRows) {
+    JoinState s[kRows];
+    join_rows<kRows, kParts>(p, parts, un.parts, 0, 1, r0, rows, lane, s);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i)
+      if (r0 + i < rows) join_store(p, un, r0 + i, lane, s[i]);
+  }
+}
+
+__global__ void __launch_bounds__(kJoinWarps * 32, 4)
 attn_plan_join_kernel(const PlanParams p) {
+  __shared__ float4 shared_acc[kJoinWarps][32];
+  __shared__ float shared_m[kJoinWarps], shared_sum[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int units = p.table[kPlanHdrUnits];
   const PlanUnit* unit = reinterpret_cast<const PlanUnit*>(p.table + p.table[kPlanHdrUnitAt]);
   const int32_t* part_list = p.table + p.table[kPlanHdrPartAt];
+  // (This kernel does not let the next one be brought up before its own end: with 512 units that left the next call's
+  // CTAs waiting on SMs of their own and cost 25 us of 75.)
+  bool waited = false;
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const PlanUnit un = unit[u];
     const int32_t* parts = part_list + un.part0;
-    for (int r = warp; r < un.n_tokens * p.group; r += kJoinWarps) {
-      const int token = r / p.group;
-      const int head = un.kv_head * p.group + (r - token * p.group);
-      float top = kNegInf;
-      for (int k = lane; k < un.parts; k += 32) top = fmaxf(top, __ldcg(p.part_lse + parts[k] + r));
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const float base = top == kNegInf ? 0.0f : top;
-      float sum = 0.0f;
-      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int k0 = 0; k0 < un.parts; k0 += 32) {
-        const int n = min(32, un.parts - k0);
-        float wgt = 0.0f;
-        int at = 0;
-        if (lane < n) {
-          at = parts[k0 + lane] + r;
-          wgt = expf(__ldcg(p.part_lse + at) - base);
-        }
-        sum += wgt;
-        for (int k = 0; k < n; k += 4) {
-          float4 a[4];
-          float ww[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int src = min(k + j, n - 1);
-            const int row = __shfl_sync(0xffffffffu, at, src);
-            ww[j] = __shfl_sync(0xffffffffu, wgt, src);
-            if (k + j >= n) ww[j] = 0.0f;
-            // a part without a visible key has weight 0 and a row of zeros
-            a[j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + int64_t(row) * kHeadDim) + lane);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (k + j < n) {
-              acc.x = fmaf(a[j].x, ww[j], acc.x);
-              acc.y = fmaf(a[j].y, ww[j], acc.y);
-              acc.z = fmaf(a[j].z, ww[j], acc.z);
-              acc.w = fmaf(a[j].w, ww[j], acc.w);
-            }
-          }
+    if (!waited) wait_for_previous();
+    waited = true;
+    const int rows = un.n_tokens * p.group;
+    if (rows <= kJoinWarps / 2 && un.parts > 2) {  // uniform across the block
+      const int per_row = rows == 1 ? 8 : rows == 2 ? 4 : 2;  // warps of a row
+      const int r = warp / per_row, share = warp - r * per_row;
+      JoinState s[1];
+      if (r < rows) {
+        join_rows<1, 4>(p, parts, un.parts, share, per_row, r, rows, lane, s);
+        shared_acc[warp][lane] = s[0].acc;
+        if (lane == 0) {
+          shared_m[warp] = s[0].m;
+          shared_sum[warp] = s[0].sum;
         }
       }
-#pragma unroll
-      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      const bool seen = sum != 0.0f;
-      const float inv = seen ? 1.0f / sum : 0.0f;
-      const int64_t row = int64_t(un.token) + token;
-      uint2 out;
-      out.x = pack_bf16x2(acc.x * inv, acc.y * inv);
-      out.y = pack_bf16x2(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>(p.o + row * p.o_stride_t + int64_t(head) * p.o_stride_h + lane * 4) = out;
-      if (p.lse != nullptr && lane == 0)
-        p.lse[int64_t(head) * p.lse_stride_h + row] = seen ? base + logf(sum) : kNegInf;
+      __syncthreads();
+      if (r < rows && share == 0) {
+        for (int j = 1; j < per_row; ++j) {
+          const float m = shared_m[warp + j], top = fmaxf(s[0].m, m);
+          s[0].rebase(top);
+          s[0].add(join_weight(m, top), shared_acc[warp + j][lane], shared_sum[warp + j]);
+        }
+        join_store(p, un, r, lane, s[0]);
+      }
+      __syncthreads();
+    } else if (un.parts <= 2) {
+      join_unit<2, 2>(p, un, parts, rows, warp, lane);
+    } else {
+      join_unit<1, 4>(p, un, parts, rows, warp, lane);
     }
   }
+  if (!waited) wait_for_previous();
 }
 
 }  // namespace
@@ -834,13 +950,11 @@ cudaError_t prepare_plan_kernels() {
 }
 
 cudaError_t launch_plan(const PlanMaps& maps, const PlanParams& p, int grid, cudaStream_t stream) {
-  attn_plan_kernel<<<grid, kPlanThreads, kPlanSmemBytes, stream>>>(maps, p);
-  return cudaGetLastError();
+  return launch_overlapped(attn_plan_kernel, grid, kPlanThreads, kPlanSmemBytes, stream, maps, p);
 }
 
 cudaError_t launch_plan_join(const PlanParams& p, int grid, cudaStream_t stream) {
-  attn_plan_join_kernel<<<grid, kJoinWarps * 32, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_overlapped(attn_plan_join_kernel, grid, kJoinWarps * 32, 0, stream, p);
 }
 
 }  // namespace b200attn

@@ -19,16 +19,17 @@ namespace {
 
 constexpr int kTile = 128;
 
-// Costs in thousandths of the time of a K/V tile against two Q tiles (about 1.6 us). A piece of one Q tile runs on
-// one of a CTA's two lanes: alone it is bound by its chain of steps, beside another lane by what the two share.
+// Costs in thousandths of the time of a K/V tile against two Q tiles (1.6 us), as measured with pieces of equal length.
+// A piece of one Q tile runs on one of a CTA's two lanes: alone it is bound by its chain of steps, beside another lane
+// by what the two share, which is above all memory (64 KB per tile).
 constexpr int64_t kTilePair = 1000;
-constexpr int64_t kPairStart = 1800;    // Q load, first scores, last PV, stores
-constexpr int64_t kTileShared = 900;    // memory and tensor pipe, per tile of a lane
-constexpr int64_t kSharedStart = 500;
+constexpr int64_t kPairStart = 2200;    // Q load, first scores, last PV, stores
+constexpr int64_t kTileShared = 930;
+constexpr int64_t kSharedStart = 750;
 constexpr int64_t kTileChain = 950;     // scores, softmax, PV of one tile after the other
-constexpr int64_t kChainStart = 1500;
-constexpr int64_t kJoin = 2200;         // the second kernel, once,
-constexpr int64_t kJoinRows = 17;       // and per row of partial results, divided by this: written, then read, by all CTAs
+constexpr int64_t kChainStart = 1300;
+constexpr int64_t kJoin = 2500;         // the second kernel, once,
+constexpr int64_t kJoinRows = 14;       // and per row of partial results, divided by this
 
 struct Item {
   int32_t token, n_tokens, kv_row, n_keys, tiles0, tiles1, diag, kv_head, source;

@@ -18,6 +18,7 @@
 // Statistics and rotation are in 32 bits and rounded to bf16 once. Angles are reduced to a fraction of a turn in
 // 64 bits first: at position 10^6 a 32-bit product is already off by 0.03 radians.
 
+#include "launch_overlap.cuh"
 #include "ptx_sm100.cuh"
 #include "rotary_kernels.cuh"
 
@@ -174,6 +175,8 @@ template <bool kInterleaved>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_norm_rope_kernel(const RotaryParams p) {
   __shared__ alignas(16) float2 turns_of[kWarps][kPairs];
   __shared__ alignas(16) float weights[2][128];  // 1 where there is none
+  launch_dependents();
+  wait_for_previous();
   for (int i = threadIdx.x; i < 256; i += kWarps * 32)
     weights[i >> 7][i & 127] = weight_of((i >> 7) ? p.k.weight : p.q.weight, p.weight_fp32, i & 127);
   __syncthreads();
@@ -227,11 +230,8 @@ cudaError_t launch_qk_norm_rope(RotaryParams p, bool interleaved, int sm_count, 
   p.chunk_heads = ((heads + chunks - 1) / chunks + 3) / 4 * 4;
   p.chunks = (heads + p.chunk_heads - 1) / p.chunk_heads;
   const int64_t blocks = (rows * p.chunks + kWarps - 1) / kWarps;
-  if (interleaved)
-    qk_norm_rope_kernel<true><<<unsigned(blocks), kWarps * 32, 0, stream>>>(p);
-  else
-    qk_norm_rope_kernel<false><<<unsigned(blocks), kWarps * 32, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_overlapped(interleaved ? qk_norm_rope_kernel<true> : qk_norm_rope_kernel<false>, unsigned(blocks),
+                           kWarps * 32, 0, stream, p);
 }
 
 }  // namespace b200attn
