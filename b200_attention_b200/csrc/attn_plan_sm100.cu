@@ -8,7 +8,7 @@
 //
 // The kernel is built like attn_fwd_ws_kernel (same tiles, descriptors, TMEM layout and softmax):
 //   warps 0-3, 4-7  softmax of Q tile 0 / 1, a row per thread
-//   warps 8-11      epilogue: bf16 O and LSE, or an fp32 partial
+//   warps 8-11      epilogue: bf16 O and LSE, or an fp32 partial (a lane's last piece: its softmax warps)
 //   warp 12         tcgen05.mma     warp 13  TMA loads
 //   warp 14         clears the rows of a V tile behind the last key: they belong to another sequence or to
 //                   memory nobody wrote, and 0 * NaN is NaN in the product P V
@@ -36,8 +36,10 @@ namespace {
 constexpr int kPairSlotsP = 2;
 constexpr int kPairBytesP = 2 * kTileBytes;
 constexpr int kPlanThreads = 512;
-constexpr int kPlanRegsSoftmax = 184;
-constexpr int kPlanRegsEpilogue = 64;
+// Registers per thread of the three kinds of warps (128 in the mean). Against 184 / 64 / 80: 3 % at 8 prompts of 1 to
+// 8192 tokens; against 192 / 56 / 72: 2 %, the MMA warp then spills.
+constexpr int kPlanRegsSoftmax = 192;
+constexpr int kPlanRegsEpilogue = 48;
 constexpr int kPlanRegsOther = 80;
 constexpr int kQSlots = 4;        // small Q tiles that a lane's buffer holds
 constexpr int kQSlotRows = 32;    // rows of each
@@ -58,6 +60,11 @@ enum PlanBarrier : int {
   kPbDrain = 34,
   kNumPlanBarriers = 35
 };
+
+__device__ __forceinline__ uint32_t plan_barrier_count(int i) {
+  if ((i >= kPbPReady && i < kPbPvDone) || (i >= kPbFin && i < kPbPairFull)) return 4;  // a warpgroup's four warps
+  return i >= kPbPairEmpty && i < kPbTailClean ? 2 : 1;
+}
 
 struct alignas(16) PlanAux {
   uint64_t bar[kNumPlanBarriers];
@@ -81,8 +88,26 @@ struct Pieces {
   __device__ __forceinline__ Pieces(const PlanParams& p, const PlanAux* a)
       : aux(a), table(reinterpret_cast<const PlanPiece*>(p.table + kPlanPieceAt) + a->first[0]),
         pairs(a->first[1] - a->first[0]), lane1(a->first[2] - a->first[0]), end(a->first[3] - a->first[0]) {}
+  __device__ __forceinline__ int last_of(int lane) const {  // -1: none
+    return lane ? (end > lane1 ? end - 1 : pairs - 1) : (lane1 > pairs ? lane1 - 1 : pairs - 1);
+  }
   __device__ __forceinline__ const PlanPiece* at(int i) const { return i < kPieceCache ? &aux->cache[i] : table + i; }
 };
+
+__device__ __forceinline__ PlanPiece piece_of(int4 a, int4 b, int4 c) {
+  PlanPiece p;
+  p.token = a.x;
+  p.n_tokens = a.y;
+  p.kv_row = a.z;
+  p.n_keys = a.w;
+  p.tiles[0] = b.x;
+  p.tiles[1] = b.y;
+  p.diag = b.z;
+  p.kv_head = b.w;
+  p.source = c.x;
+  p.slot_row = c.y;
+  return p;
+}
 
 // Steps of the pieces of one Q tile: a K/V tile of lane 0, one of lane 1, and so on; a lane that has run out leaves
 // the turns to the other.
@@ -460,6 +485,65 @@ __device__ void plan_mma_role(const PlanParams& p, const PlanAux* aux, uint32_t 
   }
 }
 
+// ---- the result of a row ---------------------------------------------------------------------------------------
+// The calling thread's row r of a Q tile: normalised O (from TMEM, `o_row`) and LSE, to o and lse or to the piece's
+// partial result. Called by whole warps; kLoads x 16 columns are read at a time.
+template <int kLoads>
+__device__ __forceinline__ void store_result(const PlanParams& p, const PlanPiece* pc, int tile, int r, float m, float l,
+                                             uint32_t o_row) {
+  const int token_in_tile = r / p.group, head_in_group = r - token_in_tile * p.group;
+  const int token = tile * p.tile_tokens + token_in_tile;  // of the block
+  const bool live = r < p.tile_rows && token < pc->n_tokens;
+  if (!__any_sync(0xffffffffu, live)) return;
+  const bool seen = l != 0.0f;  // false: the row saw no key (a NaN sum counts as seen)
+  const float weight = 1.0f / l;
+  const float lse = seen ? (m + log2f(l)) * kLn2 : kNegInf;
+  const int slot_row = pc->slot_row;
+  const int head = pc->kv_head * p.group + head_in_group;
+  const int64_t row = int64_t(pc->token) + token;
+  float* part = nullptr;
+  __nv_bfloat16* out = nullptr;
+  if (live) {
+    if (slot_row >= 0) {
+      const int64_t at = int64_t(slot_row) + token * p.group + head_in_group;
+      part = p.part_o + at * kHeadDim;
+      p.part_lse[at] = lse;
+    } else {
+      out = p.o + row * p.o_stride_t + int64_t(head) * p.o_stride_h;
+      if (p.lse != nullptr) p.lse[int64_t(head) * p.lse_stride_h + row] = lse;
+    }
+  }
+  constexpr int kChunk = 16;
+#pragma unroll 1
+  for (int c = 0; c < kHeadDim / kChunk; c += kLoads) {
+    __syncwarp();
+    uint32_t acc[kLoads][kChunk];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) tmem_ld16(o_row + (c + u) * kChunk, acc[u]);
+    tmem_wait_ld();
+    if (live) {
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        float v[kChunk];
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) v[j] = seen ? __uint_as_float(acc[u][j]) * weight : 0.0f;
+        if (slot_row >= 0) {
+          float4* dst = reinterpret_cast<float4*>(part + (c + u) * kChunk);
+#pragma unroll
+          for (int j = 0; j < kChunk / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+          uint4* dst = reinterpret_cast<uint4*>(out + (c + u) * kChunk);
+#pragma unroll
+          for (int j = 0; j < kChunk / 8; ++j)
+            dst[j] = make_uint4(pack_bf16x2(v[8 * j + 0], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                                pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+        }
+      }
+    }
+  }
+  __syncwarp();
+}
+
 // ---- softmax: one row per thread -------------------------------------------------------------------------
 // As in attn_fwd_ws_kernel: speculative against the row's reference maximum, exact where the tile's sum says that it
 // has to move. Two differences. The first tile speculates too, on a reference of 0: any reference within 2^32 of the
@@ -476,26 +560,30 @@ __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t ba
   const uint32_t p_tmem = s_tmem;  // bf16 P overwrites S columns 0..63
   const uint32_t o_tmem = tmem_base + kQTilesPerItem * kBlockN + q * kHeadDim + lane_field;
   const int r = warp_in_group * 32 + lane;
-  const int token_in_tile = min(r, p.tile_rows - 1) / p.group;  // idle rows go with the last
   const float scale_log2 = p.scale_log2;
   const f2 scale2 = f2_splat(scale_log2);
   uint32_t s_parity = 0, fin_free_parity = 1;
+  uint32_t pieces = 0;  // of this lane, so far
 
-  const Pieces ps(p, aux);
-  const int my_end = q ? ps.end : ps.lane1;
-  for (int n = 0; n < my_end; ++n) {
-    if (q && n == ps.pairs) n = ps.lane1;  // over lane 0's pieces
-    if (n >= my_end) break;
-    const PlanPiece* pc = ps.at(n);
-    const int tile = n < ps.pairs ? q : 0;  // which of the piece's Q tiles
-    const int T = pc->tiles[tile];
-    const int n_keys = pc->n_keys, diag = pc->diag + tile * p.tile_tokens;
-    // rows of this tile that exist; a warp without one only keeps the protocol going
-    const int rows = (min(pc->n_tokens - tile * p.tile_tokens, p.tile_tokens)) * p.group;
+  for (int n = 0;; ++n) {
+    int T, tile_limit, row_limit, rows;
+    {
+      // (Looked up anew for every piece: the loop over its tiles needs the registers.)
+      const Pieces ps(p, aux);
+      if (q && n == ps.pairs) n = ps.lane1;  // over lane 0's pieces
+      if (n >= (q ? ps.end : ps.lane1)) break;
+      const PlanPiece* pc = ps.at(n);
+      const int tile = n < ps.pairs ? q : 0;  // which of the piece's Q tiles
+      T = pc->tiles[tile];
+      const int n_keys = pc->n_keys, diag = pc->diag + tile * p.tile_tokens;
+      const int token_in_tile = min(r, p.tile_rows - 1) / p.group;  // idle rows go with the last
+      tile_limit = min(n_keys - 1, diag);                 // last key that the tile's first row sees
+      row_limit = min(n_keys - 1, diag + token_in_tile);  // last key that this row sees
+      // rows of this tile that exist; a warp without one only keeps the protocol going
+      rows = (min(pc->n_tokens - tile * p.tile_tokens, p.tile_tokens)) * p.group;
+    }
     const bool row_live = r < rows;
     const bool warp_live = warp_in_group * 32 < rows;
-    const int tile_limit = min(n_keys - 1, diag);                 // last key that the tile's first row sees
-    const int row_limit = min(n_keys - 1, diag + token_in_tile);  // last key that this row sees
     w.item = n;
     w.tile = 0;
     if (!w.wait_warp(bar(kPbFinFree + q), fin_free_parity, 310 + q)) return;
@@ -574,96 +662,58 @@ __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t ba
       __syncwarp();
       mbar_arrive_lead(lane == 0 ? 1u : 0u, bar(kPbPReady + q));
     }
-    aux->row_max[q][r] = m;
-    aux->row_sum[q][r] = l;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar(kPbFin + q));
+    const Pieces ps(p, aux);
+    if (n != ps.last_of(q)) {
+      aux->row_max[q][r] = m;
+      aux->row_sum[q][r] = l;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(kPbFin + q));
+    } else {
+      // This lane's last piece: these warps have nothing left to do, so they store its result themselves, both lanes at
+      // the same time. (The piece before it is through: its epilogue handed kPbFinFree back after its last PV, so the
+      // phase waited for here is the next one.)
+      if (!w.wait_warp(bar(kPbPvDone + q), pieces & 1u, 430 + q)) return;
+      tc_fence_after_sync();
+      store_result<2>(p, ps.at(n), n < ps.pairs ? q : 0, r, m, l, o_tmem);
+    }
+    ++pieces;
   }
 }
 
 // ---- epilogue -----------------------------------------------------------------------------------------------
+// Warps 8 to 11, for all but the last piece of each lane (see above).
 __device__ void plan_epilogue_role(const PlanParams& p, const PlanAux* aux, uint32_t bar0, uint32_t tmem_base,
                                    int warp_in_group, int lane, WaitCtx& w) {
   auto bar = [&](int i) { return bar0 + 8u * uint32_t(i); };
   const uint32_t lane_field = uint32_t(warp_in_group * 32) << 16;
   const int r = warp_in_group * 32 + lane;
-  const int token_in_tile = r / p.group, head_in_group = r - token_in_tile * p.group;
   uint32_t fin_parity = 0;  // bit per lane
+  const Pieces ps(p, aux);
 
-  // The result of a lane's piece: its Q tile `tile` of the piece.
-  auto finish = [&](const PlanPiece* pc, int q, int tile) -> bool {
-      if (!w.wait_warp(bar(kPbFin + q), (fin_parity >> q) & 1u, 410 + q)) return false;
-      if (!w.wait_warp(bar(kPbPvDone + q), (fin_parity >> q) & 1u, 420 + q)) return false;
-      fin_parity ^= 1u << q;
-      tc_fence_after_sync();
-      const float m = aux->row_max[q][r];
-      const float l = aux->row_sum[q][r];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kPbFinFree + q));
-      const int token = tile * p.tile_tokens + token_in_tile;  // of the block
-      const bool live = r < p.tile_rows && token < pc->n_tokens;
-      const bool any_live = __any_sync(0xffffffffu, live);
-      const bool seen = l != 0.0f;  // false: the row saw no key (a NaN sum counts as seen)
-      const float weight = 1.0f / l;
-      const float lse = seen ? (m + log2f(l)) * kLn2 : kNegInf;
-      const int slot_row = pc->slot_row;
-      const int head = pc->kv_head * p.group + head_in_group;
-      const int64_t row = int64_t(pc->token) + token;
-      float* part = nullptr;
-      __nv_bfloat16* out = nullptr;
-      if (live) {
-        if (slot_row >= 0) {
-          const int64_t at = int64_t(slot_row) + token * p.group + head_in_group;
-          part = p.part_o + at * kHeadDim;
-          p.part_lse[at] = lse;
-        } else {
-          out = p.o + row * p.o_stride_t + int64_t(head) * p.o_stride_h;
-          if (p.lse != nullptr) p.lse[int64_t(head) * p.lse_stride_h + row] = lse;
-        }
-      }
-      const uint32_t o_row = tmem_base + kQTilesPerItem * kBlockN + q * kHeadDim + lane_field;
-      constexpr int kChunk = 16;
-      if (any_live) {
-#pragma unroll 1
-        for (int c = 0; c < kHeadDim / kChunk; c += 2) {
-          uint32_t acc[2][kChunk];
-          tmem_ld16(o_row + c * kChunk, acc[0]);
-          tmem_ld16(o_row + (c + 1) * kChunk, acc[1]);
-          tmem_wait_ld();
-          if (!live) continue;
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            float v[kChunk];
-#pragma unroll
-            for (int j = 0; j < kChunk; ++j) v[j] = seen ? __uint_as_float(acc[u][j]) * weight : 0.0f;
-            if (slot_row >= 0) {
-              float4* dst = reinterpret_cast<float4*>(part + (c + u) * kChunk);
-#pragma unroll
-              for (int j = 0; j < kChunk / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-            } else {
-              uint4* dst = reinterpret_cast<uint4*>(out + (c + u) * kChunk);
-#pragma unroll
-              for (int j = 0; j < kChunk / 8; ++j)
-                dst[j] = make_uint4(pack_bf16x2(v[8 * j + 0], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                                    pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
-            }
-          }
-        }
-      }
-      // O_q has been read: the next piece's first PV may overwrite it
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kPbOFree + q));
-      return true;
+  // The result of piece n on lane q: its Q tile `tile`.
+  auto finish = [&](int n, int q, int tile) -> bool {
+    if (n == ps.last_of(q)) return true;
+    if (!w.wait_warp(bar(kPbFin + q), (fin_parity >> q) & 1u, 410 + q)) return false;
+    if (!w.wait_warp(bar(kPbPvDone + q), (fin_parity >> q) & 1u, 420 + q)) return false;
+    fin_parity ^= 1u << q;
+    tc_fence_after_sync();
+    const float m = aux->row_max[q][r];
+    const float l = aux->row_sum[q][r];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kPbFinFree + q));
+    store_result<1>(p, ps.at(n), tile, r, m, l, tmem_base + kQTilesPerItem * kBlockN + q * kHeadDim + lane_field);
+    // O_q has been read: the next piece's first PV may overwrite it
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(kPbOFree + q));
+    return true;
   };
 
-  const Pieces ps(p, aux);
   for (int n = 0; n < ps.pairs; ++n) {
-    const PlanPiece* pc = ps.at(n);
     w.item = n;
     for (int q = 0; q < kQTilesPerItem; ++q) {
-      w.tile = pc->tiles[q];
-      if (!finish(pc, q, q)) return;
+      w.tile = ps.at(n)->tiles[q];
+      if (!finish(n, q, q)) return;
     }
   }
   LaneWalk walk(ps);  // pieces end in the order of their last steps
@@ -672,7 +722,7 @@ __device__ void plan_epilogue_role(const PlanParams& p, const PlanAux* aux, uint
     if (!st.last) continue;
     w.item = st.piece;
     w.tile = st.tile;
-    if (!finish(ps.at(st.piece), st.lane, 0)) return;
+    if (!finish(st.piece, st.lane, 0)) return;
   }
 }
 
@@ -698,7 +748,9 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
   // this kernel has waited for the ones before it).
   launch_dependents();
   const bool misaligned = (smem_q & 1023u) != 0;  // uniform across the CTA
-  const int4 first = reinterpret_cast<const int4*>(p.table + kPlanCtaAt)[blockIdx.x];
+  const int4* record = reinterpret_cast<const int4*>(p.table + kPlanCtaAt + kPlanCtaWords * blockIdx.x);
+  if (warp == 13 && lane < 6) tma_prefetch_desc(&maps.q + lane);
+  const int4 first = record[0];
   const int piece0 = first.x, piece1 = first.w;
   if (misaligned || piece0 >= piece1) {  // uniform across the CTA; the latter: a table with fewer CTAs than the grid
     if (threadIdx.x == 0 && misaligned) {
@@ -711,37 +763,16 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
   const uint32_t lead = (lane == 0) ? 1u : 0u;
   Loader loader(p, maps, smem_q, smem_kv, bar0, lead);
   if (warp == 13) {
-    if (lane < 6) tma_prefetch_desc(&maps.q + lane);
-    const int4* src = reinterpret_cast<const int4*>(p.table + kPlanPieceAt) + size_t(piece0) * 3;
-    alignas(16) PlanPiece piece;
-#pragma unroll
-    for (int j = 0; j < 3; ++j) reinterpret_cast<int4*>(&piece)[j] = src[j];
+    const PlanPiece piece = piece_of(record[1], record[2], record[3]);
+    for (int i = lane; i < kNumPlanBarriers; i += 32) mbar_init(bar0 + 8u * i, plan_barrier_count(i));
+    mbar_init_fence();
+    fence_proxy_async_smem();
     if (lane == 0) {
       aux->abort_flag = 0;
       aux->first[0] = first.x;
       aux->first[1] = first.y;
       aux->first[2] = first.z;
       aux->first[3] = first.w;
-      for (int q = 0; q < kQTilesPerItem; ++q) {
-        for (int n = 0; n < kQSlots; ++n) {
-          mbar_init(bar0 + 8u * (kPbQFull + q * kQSlots + n), 1);
-          mbar_init(bar0 + 8u * (kPbQEmpty + q * kQSlots + n), 1);
-        }
-        mbar_init(bar0 + 8u * (kPbSFull + q), 1);
-        mbar_init(bar0 + 8u * (kPbPReady + q), 4);
-        mbar_init(bar0 + 8u * (kPbPvDone + q), 1);
-        mbar_init(bar0 + 8u * (kPbFin + q), 4);
-        mbar_init(bar0 + 8u * (kPbFinFree + q), 4);
-        mbar_init(bar0 + 8u * (kPbOFree + q), 4);
-      }
-      for (int s = 0; s < kPairSlotsP; ++s) {
-        mbar_init(bar0 + 8u * (kPbPairFull + s), 1);
-        mbar_init(bar0 + 8u * (kPbPairEmpty + s), 2);
-        mbar_init(bar0 + 8u * (kPbTailClean + s), 1);
-      }
-      mbar_init(bar0 + 8u * kPbDrain, 1);
-      mbar_init_fence();
-      fence_proxy_async_smem();
     }
     __syncwarp();
     // The whole CTA waits here (at the barrier below), before any of its bounded waits begin.
@@ -903,7 +934,10 @@ attn_plan_join_kernel(const PlanParams p) {
   for (int u = blockIdx.x; u < units; u += gridDim.x) {
     const PlanUnit un = unit[u];
     const int32_t* parts = part_list + un.part0;
-    if (!waited) wait_for_previous();
+    if (!waited) {
+      if (lane < un.parts) asm volatile("prefetch.global.L1 [%0];" ::"l"(parts + lane));
+      wait_for_previous();
+    }
     waited = true;
     const int rows = un.n_tokens * p.group;
     if (rows <= kJoinWarps / 2 && un.parts > 2) {  // uniform across the block

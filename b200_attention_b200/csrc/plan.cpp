@@ -25,7 +25,7 @@ constexpr int kTile = 128;
 constexpr int64_t kTilePair = 1000;
 constexpr int64_t kPairStart = 2200;    // Q load, first scores, last PV, stores
 constexpr int64_t kTileShared = 930;
-constexpr int64_t kSharedStart = 750;
+constexpr int64_t kSharedStart = 1000;
 constexpr int64_t kTileChain = 950;     // scores, softmax, PV of one tile after the other
 constexpr int64_t kChainStart = 1300;
 constexpr int64_t kJoin = 2500;         // the second kernel, once,
@@ -216,11 +216,13 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   if (!items.empty()) {
     std::vector<int32_t> lens{std::max(longest, 1)};
     auto consider = [&](int64_t len) {
-      len = std::max<int64_t>(2, len);
+      len = std::max<int64_t>(1, len);
       if (len < longest && std::find(lens.begin(), lens.end(), int32_t(len)) == lens.end()) lens.push_back(int32_t(len));
     };
     const int64_t even = (total_tiles + in.sm_count - 1) / in.sm_count;
     for (const int64_t parts : {1, 2, 3, 4, 6, 8}) consider((even + parts - 1) / parts);
+    consider((longest + 1) / 2);
+    consider((3 * int64_t(longest) + 3) / 4);
     // as many pieces of the longest items as fill the CTAs, or their lanes, a whole number of times
     int64_t long_items = 0;
     for (const Item& it : items) long_items += 2 * it.longest() > longest ? 1 : 0;
@@ -365,11 +367,13 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   int32_t k = 0;
   for (int32_t c = 0; c < kPlanMaxCtas; ++c) {
     for (int32_t part = 0; part < 3; ++part) {
-      t[kPlanCtaAt + 4 * c + part] = k;
+      t[kPlanCtaAt + kPlanCtaWords * c + part] = k;
       if (c < in.sm_count)
         for (const int32_t i : dealt[size_t(c) * 3 + size_t(part)]) out[k++] = pieces[size_t(i)].p;
     }
-    t[kPlanCtaAt + 4 * c + 3] = k;
+    const int32_t begin = t[kPlanCtaAt + kPlanCtaWords * c];
+    t[kPlanCtaAt + kPlanCtaWords * c + 3] = k;
+    if (begin < k) *reinterpret_cast<PlanPiece*>(t + kPlanCtaAt + kPlanCtaWords * c + 4) = out[begin];
   }
   std::copy(units.begin(), units.end(), reinterpret_cast<PlanUnit*>(t + unit_at));
   std::copy(parts.begin(), parts.end(), t + part_at);

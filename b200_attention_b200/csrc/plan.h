@@ -37,12 +37,14 @@ struct alignas(16) PlanUnit {
 static_assert(sizeof(PlanUnit) == 32, "table layout");
 
 // The table as the kernels see it, in 32-bit words: header, the pieces of every CTA as four bounds
-// (pieces of two Q tiles, then lane 0's, then lane 1's, end), pieces, units, parts (the row of the partials that holds the unit's first token, head 0 of the group).
+// (pieces of two Q tiles, then lane 0's, then lane 1's, end) with its first piece beside them, so that the loads of
+// that can start after one look at the table, pieces, units, parts (the row of the partials that holds the unit's first token, head 0 of the group).
 constexpr int kPlanMaxCtas = 160;
-constexpr int kPlanMagic = 0x62706c32;
+constexpr int kPlanMagic = 0x62706c33;
 enum PlanHeader : int { kPlanHdrMagic = 0, kPlanHdrPieces, kPlanHdrUnits, kPlanHdrUnitAt, kPlanHdrPartAt, kPlanHeaderWords = 16 };
 constexpr int kPlanCtaAt = kPlanHeaderWords;
-constexpr int kPlanPieceAt = kPlanCtaAt + 4 * kPlanMaxCtas;
+constexpr int kPlanCtaWords = 16;  // the bounds, and a copy of the CTA's first piece
+constexpr int kPlanPieceAt = kPlanCtaAt + kPlanCtaWords * kPlanMaxCtas;
 
 constexpr int kPlanJoinRows = 32;  // most rows of a join unit (one token at least)
 constexpr int32_t kPlanNoDiag = 1 << 30;

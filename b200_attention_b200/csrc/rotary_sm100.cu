@@ -220,13 +220,11 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_norm_rope_kernel
 cudaError_t launch_qk_norm_rope(RotaryParams p, bool interleaved, int sm_count, cudaStream_t stream) {
   const int64_t rows = int64_t(p.batch) * p.tokens;
   const int heads = p.heads_q + p.heads_k;
-  // With few tokens a token's heads are spread over several warps (each works the angles out again).
-  const int64_t wanted = int64_t(sm_count) * 32;
+  // With few tokens a token's heads are spread over several warps (each works the angles out again), as far as all
+  // warps are still resident at once.
+  const int64_t resident = int64_t(sm_count) * kBlocksPerSm * kWarps, most = (heads + 3) / 4;
   int chunks = 1;
-  if (rows < wanted) {
-    const int64_t most = (heads + 3) / 4;
-    chunks = int((wanted + rows - 1) / rows < most ? (wanted + rows - 1) / rows : most);
-  }
+  if (rows * 2 <= resident) chunks = int(resident / rows < most ? resident / rows : most);
   p.chunk_heads = ((heads + chunks - 1) / chunks + 3) / 4 * 4;
   p.chunks = (heads + p.chunk_heads - 1) / p.chunk_heads;
   const int64_t blocks = (rows * p.chunks + kWarps - 1) / kWarps;

@@ -11,7 +11,7 @@ import torch
 from b200_attention_b200 import _native as N
 from b200_attention_b200 import ops, packed
 
-CTA_AT, PIECE_AT = 16, 656  # words: bounds of each CTA's pieces (two Q tiles, lane 0, lane 1, end), pieces
+CTA_AT, PIECE_AT = 16, 2576  # words: a record for each CTA (bounds of its pieces and a copy of the first), pieces
 
 
 def expand(lens_q, lens_kv, heads, heads_kv, *, causal, starts=None, prefix=0, sm_count=0):
@@ -21,7 +21,8 @@ def expand(lens_q, lens_kv, heads, heads_kv, *, causal, starts=None, prefix=0, s
     t, info = s.table.numpy(), s.info
     group = heads // heads_kv
     per_tile = 128 // group
-    ctas = t[CTA_AT:PIECE_AT].reshape(160, 4)
+    records = t[CTA_AT:PIECE_AT].reshape(160, 16)
+    ctas = records[:, :4]  # pieces of two Q tiles, lane 0's, lane 1's, end
     assert ctas[0, 0] == 0 and ctas[-1, 3] == info.pieces == t[1] and (np.diff(ctas.ravel()) >= 0).all()
     assert (ctas[1:, 0] == ctas[:-1, 3]).all()
     assert (ctas[info.grid:, 0] == info.pieces).all() and info.grid <= (sm_count or 148)
@@ -29,6 +30,8 @@ def expand(lens_q, lens_kv, heads, heads_kv, *, causal, starts=None, prefix=0, s
     pieces = t[PIECE_AT:PIECE_AT + 12 * info.pieces].reshape(-1, 12)
     units = t[t[3]:t[3] + 8 * info.units].reshape(-1, 8)
     parts = t[t[4]:]
+    for record in records[ctas[:, 0] < ctas[:, 3]]:
+        assert (record[4:] == pieces[record[0]]).all()
     both = pieces[:, 5] > 0
     for pairs, lane0, lane1, end in ctas.tolist():
         assert both[pairs:lane0].all() and not both[lane0:end].any()
@@ -133,7 +136,7 @@ def test_work_is_spread_evenly(native_built):
         s = packed.Schedule(lens_q, lens_kv, heads=heads, heads_kv=heads_kv)
         t = s.table.numpy()
         pieces = t[PIECE_AT:PIECE_AT + 12 * s.info.pieces].reshape(-1, 12)
-        ctas = t[CTA_AT:PIECE_AT].reshape(160, 4)
+        ctas = t[CTA_AT:PIECE_AT].reshape(160, 16)
         tiles = pieces[:, 4:6].max(1)
         load = [tiles[a:b].sum() for a, b in ctas[:148, [0, 3]]]
         assert max(load) <= np.mean(load) + 2 * s.info.pieces / 148 + tiles.max() + 2
