@@ -14,6 +14,7 @@ LIB_DIR = PKG / "lib"
 CORE_LIB = LIB_DIR / "libb200attn.so"
 TORCH_LIB = LIB_DIR / "libb200attn_torch.so"
 LTX_LIB = LIB_DIR / "libltx_sm100_attention.so"
+DIRECT_LIB = LIB_DIR / "_direct.so"
 
 KERNEL_WARP_SPECIALIZED = 0
 KERNEL_SERIAL = 1
@@ -264,6 +265,29 @@ def torch_ops():
         torch.ops.load_library(str(TORCH_LIB))
         _torch_ops = torch.ops.b200_attention_b200
     return _torch_ops
+
+
+_direct = None
+
+
+def direct():
+    """The module of lib/_direct.so (packed, shared-prefix and rotation calls), loaded once; raises if it has not been
+    built."""
+    global _direct
+    if _direct is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (the module links against it)
+
+        lib()
+        if not DIRECT_LIB.exists():
+            raise ImportError(f"{DIRECT_LIB} is missing: run `python -m b200_attention_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_direct", str(DIRECT_LIB))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_direct", loader))
+        loader.exec_module(module)
+        _direct = module
+    return _direct
 
 
 def check(status: int) -> None:

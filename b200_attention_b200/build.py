@@ -7,6 +7,7 @@ Outputs (git-ignored, next to the sources they come from):
     b200_attention_b200/lib/libb200attn.so              kernels + C ABI (no torch dependency)
     b200_attention_b200/lib/libb200attn_torch.so        torch ops `b200_attention_b200::*`
     b200_attention_b200/lib/libltx_sm100_attention.so   torch op  `ltx_sm100::attention`
+    b200_attention_b200/lib/_direct.so                  Python module behind packed.py and rotary.py
 """
 
 from __future__ import annotations
@@ -16,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -91,9 +93,12 @@ def _torch_flags():
     return cflags, ldflags, torch.__version__
 
 
-def _build_torch_lib(src: Path, out: Path, force: bool, verbose: bool) -> Path:
+def _build_torch_lib(src: Path, out: Path, force: bool, verbose: bool, python: bool = False) -> Path:
     cflags, ldflags, tver = _torch_flags()
-    digest = _digest([src, INCLUDE / "b200_attention.h"], tver + " ".join(cflags))
+    if python:
+        cflags = [*cflags, f"-I{sysconfig.get_paths()['include']}", "-fvisibility=hidden"]
+        ldflags = [*ldflags, "-ltorch_python"]
+    digest = _digest([src, CSRC / "serving_calls.h", INCLUDE / "b200_attention.h"], tver + " ".join(cflags))
     if force or _stale(out, digest):
         _run([os.environ.get("CXX", "g++"), *cflags, "-o", out, src, *ldflags], verbose)
         out.with_suffix(".so.sha256").write_text(digest)
@@ -103,6 +108,11 @@ def _build_torch_lib(src: Path, out: Path, force: bool, verbose: bool) -> Path:
 def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
     build_core(False, verbose)
     return _build_torch_lib(CSRC / "torch_ops.cpp", LIB / "libb200attn_torch.so", force, verbose)
+
+
+def build_direct(force: bool = False, verbose: bool = False) -> Path:
+    build_core(False, verbose)
+    return _build_torch_lib(CSRC / "direct.cpp", LIB / "_direct.so", force, verbose, python=True)
 
 
 def build_ltx_op(force: bool = False, verbose: bool = False) -> Path:
@@ -115,6 +125,7 @@ def build_all(force: bool = False, verbose: bool = False) -> dict[str, Path]:
         "core": build_core(force, verbose),
         "torch_ops": build_torch_ops(force, verbose),
         "ltx_op": build_ltx_op(force, verbose),
+        "direct": build_direct(force, verbose),
     }
 
 

@@ -1,0 +1,225 @@
+// Tensor-level bodies of the packed, shared-prefix and norm-and-rotation calls: argument rules, outputs, workspace, launch.
+// Behind the torch ops (torch_ops.cpp) and behind b200_attention_b200.packed and .rotary (direct.cpp).
+#pragma once
+
+#include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+
+#include <limits>
+#include <optional>
+#include <tuple>
+
+#include "../../include/b200_attention.h"
+
+namespace b200attn_torch {
+
+inline void check_rc(int rc) {
+  TORCH_CHECK(rc == B200ATTN_OK, "b200attn: ", b200attn_status_string(rc), ": ",
+              b200attn_last_error());
+}
+
+inline void check_bf16(const char* name, const at::Tensor& t) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (this library has no CPU path)");
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16, got ", t.scalar_type());
+  TORCH_CHECK(!(t.requires_grad() && c10::GradMode::is_enabled()), name,
+              " requires grad: this library computes forward passes only");
+}
+
+inline void check_rows(const char* name, const at::Tensor& t, int64_t heads, const at::Device& device) {
+  check_bf16(name, t);
+  TORCH_CHECK(t.dim() == 3 && t.size(2) == 128, name, " must be [rows, heads, 128], got ", t.sizes());
+  TORCH_CHECK(t.stride(2) == 1, name, ": the head_dim axis must be contiguous");
+  TORCH_CHECK(t.size(1) == heads, name, " has ", t.size(1), " heads, the plan ", heads);
+  TORCH_CHECK(t.device() == device, name, " is on ", t.device(), ", the plan on ", device);
+  TORCH_CHECK(t.size(0) < (int64_t(1) << 31) - 256, name, " has too many rows");
+}
+
+inline b200attn_operand row_operand(const at::Tensor& t) { return {t.data_ptr(), 0, t.stride(1), t.stride(0)}; }
+
+// plan: heads, heads_kv, rows_q, rows_kv, len_prefix, grid, join units, slot rows
+inline std::tuple<at::Tensor, at::Tensor> attention_planned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                     const std::optional<at::Tensor>& k_prefix,
+                                                     const std::optional<at::Tensor>& v_prefix, const at::Tensor& table,
+                                                     at::IntArrayRef plan, double scale, bool return_lse,
+                                                     const std::optional<at::Tensor>& out) {
+  TORCH_CHECK(plan.size() == 8, "malformed plan");
+  const int64_t heads = plan[0], heads_kv = plan[1], rows_q = plan[2], rows_kv = plan[3], len_prefix = plan[4];
+  const int64_t slots = plan[7];
+  const at::Device device = table.device();
+  check_rows("q", q, heads, device);
+  check_rows("k", k, heads_kv, device);
+  check_rows("v", v, heads_kv, device);
+  TORCH_CHECK(k.size(0) == v.size(0), "k has ", k.size(0), " rows, v ", v.size(0));
+  TORCH_CHECK(q.size(0) >= rows_q, "q has ", q.size(0), " rows, the plan covers ", rows_q);
+  TORCH_CHECK(k.size(0) >= rows_kv, "k and v have ", k.size(0), " rows, the plan reads up to row ", rows_kv);
+  if (len_prefix > 0) {
+    TORCH_CHECK(k_prefix.has_value() && v_prefix.has_value(), "the plan has a prefix");
+    check_rows("k_prefix", *k_prefix, heads_kv, device);
+    check_rows("v_prefix", *v_prefix, heads_kv, device);
+    TORCH_CHECK(k_prefix->size(0) >= len_prefix && v_prefix->size(0) >= len_prefix,
+                "k_prefix or v_prefix has fewer than the plan's ", len_prefix, " rows");
+  }
+  if (out.has_value()) {
+    TORCH_CHECK(out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && out->device() == device &&
+                    out->stride(2) == 1,
+                "out must match q in shape, dtype and device with a dense head_dim axis");
+    check_bf16("out", *out);
+  }
+
+  c10::cuda::CUDAGuard guard(device);
+  const int64_t rows = q.size(0);
+  at::Tensor o = out.has_value() ? *out : at::empty({rows, heads, 128}, q.options());
+  at::Tensor lse;
+  if (return_lse) lse = at::empty({heads, rows}, q.options().dtype(at::kFloat));
+  if (rows > rows_q) {
+    if (!out.has_value()) o.narrow(0, rows_q, rows - rows_q).zero_();
+    if (return_lse) lse.narrow(1, rows_q, rows - rows_q).fill_(-std::numeric_limits<float>::infinity());
+  }
+  if (rows == 0 || (plan[5] == 0 && plan[6] == 0)) return {o, lse};
+  // From the caching allocator at every call: in stream order, and private to a graph that is being captured.
+  at::Tensor workspace;
+  if (slots > 0) workspace = at::empty({slots * 129}, q.options().dtype(at::kFloat));
+  b200attn_planned_args a{};
+  a.struct_bytes = sizeof a;
+  a.heads = int32_t(heads);
+  a.heads_kv = int32_t(heads_kv);
+  a.head_dim = 128;
+  a.rows_q = int32_t(rows);
+  a.rows_kv = int32_t(k.size(0));
+  a.len_prefix = int32_t(len_prefix);
+  a.grid = int32_t(plan[5]);
+  a.join_units = int32_t(plan[6]);
+  a.q = row_operand(q);
+  a.k = row_operand(k);
+  a.v = row_operand(v);
+  if (len_prefix > 0) {
+    a.k_prefix = row_operand(*k_prefix);
+    a.v_prefix = row_operand(*v_prefix);
+  }
+  a.o = row_operand(o);
+  if (return_lse) {
+    a.lse = lse.data_ptr<float>();
+    a.lse_stride_head = rows;
+  }
+  a.softmax_scale = float(scale);
+  a.table = table.data_ptr();
+  a.workspace = slots > 0 ? workspace.data_ptr() : nullptr;
+  a.slot_rows = slots;
+  a.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  check_rc(b200attn_forward_planned(&a));
+  return {o, lse};
+}
+
+inline void check_tokens(const char* name, const at::Tensor& t, const at::Tensor* like) {
+  check_bf16(name, t);
+  TORCH_CHECK((t.dim() == 3 || t.dim() == 4) && t.size(-1) == 128, name,
+              " must be [tokens, heads, 128] or [batch, tokens, heads, 128], got ", t.sizes());
+  TORCH_CHECK(t.stride(-1) == 1, name, ": the head_dim axis must be contiguous");
+  if (like != nullptr) {
+    TORCH_CHECK(t.device() == like->device(), name, " is on ", t.device(), ", q on ", like->device());
+    TORCH_CHECK(t.dim() == like->dim() && t.sizes().slice(0, t.dim() - 2) == like->sizes().slice(0, t.dim() - 2), name,
+                " and q disagree on batch or tokens: ", t.sizes(), ", ", like->sizes());
+  }
+}
+
+// (batch, head, token); an axis of one entry is never stepped along
+inline b200attn_operand token_operand(const at::Tensor& t) {
+  auto step = [&](int64_t d) { return t.size(d) == 1 ? int64_t(0) : t.stride(d); };
+  return {t.data_ptr(), t.dim() == 4 ? step(0) : 0, step(-2), step(-3)};
+}
+
+inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, const std::optional<at::Tensor>& k,
+                                                const at::Tensor& positions, const at::Tensor& inv_freq,
+                                                at::IntArrayRef sections, const std::optional<at::Tensor>& q_weight,
+                                                const std::optional<at::Tensor>& k_weight, double eps, bool interleaved,
+                                                const std::optional<at::Tensor>& q_out,
+                                                const std::optional<at::Tensor>& k_out) {
+  check_tokens("q", q, nullptr);
+  if (k.has_value()) check_tokens("k", *k, &q);
+  TORCH_CHECK(k.has_value() || !k_weight.has_value(), "k_weight is given without k");
+  const int64_t batch = q.dim() == 4 ? q.size(0) : 1, tokens = q.size(-3);
+  TORCH_CHECK(positions.device() == q.device() && inv_freq.device() == q.device(),
+              "positions and inv_freq must be on q's device");
+  TORCH_CHECK(inv_freq.dim() == 1 && inv_freq.scalar_type() == at::kFloat && inv_freq.is_contiguous(),
+              "inv_freq must be a contiguous fp32 vector");
+  TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong ||
+                  positions.scalar_type() == at::kFloat,
+              "positions must be int32, int64 or float32, got ", positions.scalar_type());
+  const int64_t axes = int64_t(sections.size());
+  const at::Tensor pos = positions.dim() == 1 ? positions.unsqueeze(0) : positions;
+  TORCH_CHECK((pos.dim() == 2 && pos.size(0) == axes && pos.size(1) == tokens) ||
+                  (pos.dim() == 3 && pos.size(0) == axes && pos.size(1) == batch && pos.size(2) == tokens),
+              "positions must be [", axes, ", ", tokens, "] or [", axes, ", ", batch, ", ", tokens, "], got ",
+              positions.sizes());
+  TORCH_CHECK(!((positions.requires_grad() || inv_freq.requires_grad()) && c10::GradMode::is_enabled()),
+              "positions or inv_freq requires grad: this library computes forward passes only");
+  const at::Tensor* weight[2] = {q_weight.has_value() ? &*q_weight : nullptr, k_weight.has_value() ? &*k_weight : nullptr};
+  for (const at::Tensor* w : weight) {
+    if (w == nullptr) continue;
+    TORCH_CHECK(w->device() == q.device() && w->dim() == 1 && w->size(0) == 128 && w->is_contiguous() &&
+                    (w->scalar_type() == at::kBFloat16 || w->scalar_type() == at::kFloat),
+                "a weight must be a contiguous bf16 or fp32 vector of 128 on q's device");
+    TORCH_CHECK(!(w->requires_grad() && c10::GradMode::is_enabled()),
+                "a weight requires grad: this library computes forward passes only");
+  }
+  TORCH_CHECK(weight[0] == nullptr || weight[1] == nullptr || weight[0]->scalar_type() == weight[1]->scalar_type(),
+              "q_weight and k_weight must have the same type");
+  const at::Tensor* given[2] = {q_out.has_value() ? &*q_out : nullptr, k_out.has_value() ? &*k_out : nullptr};
+  if (given[0] != nullptr) {
+    check_tokens("out of q", *given[0], &q);
+    TORCH_CHECK(given[0]->sizes() == q.sizes(), "out of q must match q in shape");
+  }
+  if (given[1] != nullptr && k.has_value()) {
+    check_tokens("out of k", *given[1], &q);
+    TORCH_CHECK(given[1]->sizes() == k->sizes(), "out of k must match k in shape");
+  }
+
+  c10::cuda::CUDAGuard guard(q.device());
+  const at::Tensor qo = given[0] != nullptr ? *given[0] : at::empty(q.sizes(), q.options());
+  at::Tensor ko;
+  if (k.has_value()) ko = given[1] != nullptr ? *given[1] : at::empty(k->sizes(), k->options());
+  if (batch * tokens == 0 || q.size(-2) == 0) return {qo, ko};
+  TORCH_CHECK(batch * tokens < (int64_t(1) << 31) && q.size(-2) < (1 << 16) && (!k.has_value() || k->size(-2) < (1 << 16)),
+              "too many tokens or heads");
+  TORCH_CHECK(axes >= 1 && axes <= 4, "there must be one to four sections");
+  b200attn_qk_norm_rope_args a{};
+  a.struct_bytes = sizeof a;
+  a.batch = int32_t(batch);
+  a.tokens = int32_t(tokens);
+  a.heads_q = int32_t(q.size(-2));
+  a.head_dim = 128;
+  a.q = token_operand(q);
+  a.q_out = token_operand(qo);
+  if (k.has_value() && k->size(-2) > 0) {
+    a.heads_k = int32_t(k->size(-2));
+    a.k = token_operand(*k);
+    a.k_out = token_operand(ko);
+  }
+  a.q_weight = weight[0] != nullptr ? weight[0]->data_ptr() : nullptr;
+  a.k_weight = weight[1] != nullptr ? weight[1]->data_ptr() : nullptr;
+  const at::Tensor* any_weight = weight[0] != nullptr ? weight[0] : weight[1];
+  a.weight_type = any_weight != nullptr && any_weight->scalar_type() == at::kFloat ? 1 : 0;
+  a.position_type = pos.scalar_type() == at::kInt ? 0 : pos.scalar_type() == at::kLong ? 1 : 2;
+  a.positions = pos.data_ptr();
+  a.position_stride_axis = pos.stride(0);
+  a.position_stride_batch = pos.dim() == 3 ? pos.stride(1) : 0;
+  a.position_stride_token = pos.stride(-1);
+  a.inv_freq = inv_freq.data_ptr<float>();
+  a.axes = int32_t(axes);
+  int64_t pairs = 0;
+  for (int64_t i = 0; i < axes; ++i) {
+    TORCH_CHECK(sections[size_t(i)] >= 0 && sections[size_t(i)] <= 64, "sections must be 0 .. 64 pairs");
+    a.section[i] = int32_t(sections[size_t(i)]);
+    pairs += sections[size_t(i)];
+  }
+  TORCH_CHECK(inv_freq.size(0) == pairs, "inv_freq holds ", inv_freq.size(0), " frequencies, sections add up to ", pairs);
+  a.eps = float(eps);
+  a.interleaved = interleaved ? 1 : 0;
+  a.stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
+  check_rc(b200attn_qk_norm_rope(&a));
+  return {qo, ko};
+}
+
+}  // namespace b200attn_torch

@@ -125,11 +125,11 @@ class AttentionPlan:
             torch.cuda.current_stream().synchronize()
         i = s.info
         self.rows_q, self.rows_kv = i.rows_q, i.rows_kv
-        self._now = [self.heads, self.heads_kv, i.rows_q, i.rows_kv, self.len_prefix, i.grid, i.units, i.slot_rows]
+        self._now = (self.heads, self.heads_kv, i.rows_q, i.rows_kv, self.len_prefix, i.grid, i.units, i.slot_rows)
 
-    def _for_capture(self, k) -> list:
-        grid = self._sm_count if k.size(0) or self.len_prefix else 0
-        return self._now[:5] + [grid, self._room_units, self._room_slots]
+    def _for_capture(self, k) -> tuple:
+        grid = self._sm_count if self.len_prefix or k.size(0) else 0
+        return (*self._now[:5], grid, self._room_units, self._room_slots)
 
     def _hold(self, rows_q: int, rows_kv: int) -> None:
         held = self._captured or (rows_q, rows_kv)
@@ -156,19 +156,14 @@ class AttentionPlan:
 
 
 def _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream):
-    if not isinstance(plan, AttentionPlan):
-        raise TypeError("plan must be an AttentionPlan")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
     if stream is not None and stream != torch.cuda.current_stream(plan.device):
         with torch.cuda.stream(stream):
             return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
     # a replay may find the table of other lengths: a captured call launches for all that may be in it
     capturing = torch.cuda.is_current_stream_capturing()
-    o, lse = N.torch_ops().attention_planned(q, k, v, k_prefix, v_prefix, plan._table,
-                                             plan._for_capture(k) if capturing else plan._now, softmax_scale,
-                                             return_lse, out)
+    o, lse = (N._direct or N.direct()).attention_planned(
+        q, k, v, k_prefix, v_prefix, plan._table, plan._for_capture(k) if capturing else plan._now, softmax_scale,
+        return_lse, out)
     if capturing:
         plan._hold(q.size(0), k.size(0))
     return (o, lse) if return_lse else o
@@ -186,7 +181,9 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
     k and v outside the plan's sequences have no influence, whatever they hold. `out` must not overlap k or v.
     Forward only. softmax_scale <= 0: 1 / sqrt(128).
     """
-    if isinstance(plan, AttentionPlan) and plan.len_prefix:
+    if not isinstance(plan, AttentionPlan):
+        raise TypeError("plan must be an AttentionPlan")
+    if plan.len_prefix:
         raise RuntimeError("this plan has a prefix: use attention_shared_prefix")
     return _run(q, k, v, None, None, plan, softmax_scale, return_lse, out, stream)
 
@@ -203,9 +200,8 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         raise TypeError("plan must be an AttentionPlan")
     if not plan.len_prefix:
         raise RuntimeError("this plan has no prefix: use attention_packed")
-    for name, t in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
+    if k_prefix is None or v_prefix is None:
+        raise TypeError("k_prefix and v_prefix must be torch.Tensors")
     return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
     # a replay may find the table of other lengths: a captured call launches for all that may be in it
     capturing = torch.cuda.is_current_stream_capturing()
@@ -229,7 +225,9 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
     k and v outside the plan's sequences have no influence, whatever they hold. `out` must not overlap k or v.
     Forward only. softmax_scale <= 0: 1 / sqrt(128).
     """
-    if isinstance(plan, AttentionPlan) and plan.len_prefix:
+    if not isinstance(plan, AttentionPlan):
+        raise TypeError("plan must be an AttentionPlan")
+    if plan.len_prefix:
         raise RuntimeError("this plan has a prefix: use attention_shared_prefix")
     return _run(q, k, v, None, None, plan, softmax_scale, return_lse, out, stream)
 
@@ -246,9 +244,8 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         raise TypeError("plan must be an AttentionPlan")
     if not plan.len_prefix:
         raise RuntimeError("this plan has no prefix: use attention_packed")
-    for name, t in (("k_prefix", k_prefix), ("v_prefix", v_prefix)):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
+    if k_prefix is None or v_prefix is None:
+        raise TypeError("k_prefix and v_prefix must be torch.Tensors")
         if t.dim() < 1 or t.size(0) < plan.len_prefix:
             raise RuntimeError(f"{name} has fewer than the plan's {plan.len_prefix} rows")
     return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream)

@@ -49,6 +49,9 @@ def _dense_apart(t: torch.Tensor) -> bool:
 
 
 def _check_out(q, k, q_out, k_out) -> None:
+    for name, t, needed in (("q", q, True), ("k", k, False)):
+        if not isinstance(t, torch.Tensor) and (needed or t is not None):
+            raise TypeError(f"{name} must be a torch.Tensor")
     pairs = [("q", q, q_out)] + ([("k", k, k_out)] if k is not None else [])
     for name, src, dst in pairs:
         if not isinstance(dst, torch.Tensor):
@@ -92,18 +95,17 @@ def qk_norm_rope(
     q_weight, k_weight: [128], both bf16 or both fp32, or None (no norm). Inputs need strides that are multiples of 8
     elements. `out`: tensors to write (may be q and k themselves). One rounding to bf16, at the end. Forward only.
     """
-    for name, t, needed in (("q", q, True), ("k", k, False), ("positions", positions, True), ("inv_freq", inv_freq, True),
-                            ("q_weight", q_weight, False), ("k_weight", k_weight, False)):
-        if not isinstance(t, torch.Tensor) and (needed or t is not None):
-            raise TypeError(f"{name} must be a torch.Tensor")
     if sections is None:
         sections = (inv_freq.numel(),)
+    elif type(sections) is not tuple:
+        sections = tuple(sections)
     if not 1 <= len(sections) <= 4 or min(sections) < 0 or not 1 <= sum(sections) <= HEAD_DIM // 2:
-        raise ValueError(f"sections must be 1 to 4 counts that add up to 1 .. {HEAD_DIM // 2}, got {tuple(sections)}")
+        raise ValueError(f"sections must be 1 to 4 counts that add up to 1 .. {HEAD_DIM // 2}, got {sections}")
     if inv_freq.numel() != sum(sections):
         raise ValueError(f"inv_freq holds {inv_freq.numel()} frequencies, sections add up to {sum(sections)}")
-    q_out, k_out = (None, None) if out is None else out
+    q_out = k_out = None
     if out is not None:
+        q_out, k_out = out
         _check_out(q, k, q_out, k_out)
     if stream is not None and stream != torch.cuda.current_stream(q.device):
         with torch.cuda.stream(stream):
@@ -112,9 +114,11 @@ def qk_norm_rope(
 
 
 def _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out):
-    qo, ko = N.torch_ops().qk_norm_rope(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out,
-                                        k_out)
-    return qo if q_out is None else q_out, None if k is None else ko if k_out is None else k_out
+    done = (N._direct or N.direct()).qk_norm_rope(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved,
+                                                 q_out, k_out)
+    if q_out is None:
+        return done
+    return q_out, k_out if k is not None else None
 
 
 __all__ = ["qk_norm_rope"]
