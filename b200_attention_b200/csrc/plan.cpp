@@ -3,10 +3,11 @@
 //
 // An item is a block of 2 * floor(128 / group) tokens of one sequence and one K/V head with every
 // key it sees (for a shared prefix: a block of tokens of all sequences with the prefix). Items are
-// dealt to the CTA that is free first, longest first. Where that leaves CTAs idle at the end (few
-// or very unequal items) long items are cut into pieces of equal length first; the price of a cut is the
-// piece's own start and the join of the partial results. Which length is chosen is decided by
-// working out the finishing time for a handful of lengths.
+// dealt to the CTA that is free first, longest first. Where that leaves CTAs idle at the end, cutting helps, at the
+// price of the pieces' own starts and of the join of their partial results. Two ways of cutting are tried, and the
+// schedule that finishes first by the costs below is taken: long items into pieces of equal length, for a
+// handful of lengths (few items, single tokens with many keys); and, of a schedule with more items than CTAs, only
+// what the busiest CTAs have too much, which goes to those that have least.
 #include "plan.h"
 
 #include <algorithm>
@@ -30,6 +31,7 @@ constexpr int64_t kTileChain = 950;     // scores, softmax, PV of one tile after
 constexpr int64_t kChainStart = 1300;
 constexpr int64_t kJoin = 2500;         // the second kernel, once,
 constexpr int64_t kJoinRows = 14;       // and per row of partial results, divided by this
+constexpr int32_t kShortestCut = 3;     // tiles of what is left, and of what is taken, where an item is trimmed
 
 struct Item {
   int32_t token, n_tokens, kv_row, n_keys, tiles0, tiles1, diag, kv_head, source;
@@ -48,7 +50,7 @@ Cost cost_of(const PlanPiece& p, int32_t small_tokens) {
           kChainStart + p.tiles[0] * kTileChain};
 }
 
-// Piece `c` of an item cut every `len` tiles.
+// Tiles [from, from + len) of an item.
 PlanPiece cut_piece(const Item& it, int32_t from, int32_t len) {
   PlanPiece p{};
   p.token = it.token;
@@ -65,59 +67,184 @@ PlanPiece cut_piece(const Item& it, int32_t from, int32_t len) {
   return p;
 }
 
-int32_t cuts_of(const Item& it, int32_t len) { return (it.longest() + len - 1) / len; }
+struct Cta {
+  int64_t pairs = 0, shared = 0, lane[2] = {0, 0};
+  int64_t end() const { return pairs + std::max(shared, std::max(lane[0], lane[1])); }
+  // by the shared time: a CTA with one busy lane takes a second piece almost for nothing
+  int64_t free_at() const { return pairs + std::max(shared, std::min(lane[0], lane[1])); }
+};
 
-// Length of an item's pieces when none may exceed `len`: as equal as possible.
-int32_t even_len(const Item& it, int32_t len) {
-  const int32_t n = cuts_of(it, len);
-  return (it.longest() + n - 1) / n;
-}
+// Tiles [from, from + len) of an item.
+struct Run {
+  int32_t item, from, len;
+  Cost cost;
+};
 
-// Deals pieces (longest first, in the order given) to the CTA that is free first, and pieces of one Q tile to the
-// lane of it that is. Returns when the last CTA finishes.
-struct Dealer {
-  using Load = std::pair<int64_t, int32_t>;  // (busy until, CTA)
-  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> free;
-  struct Cta {
-    int64_t pairs = 0, shared = 0, lane[2] = {0, 0};
-    int64_t end() const { return pairs + std::max(shared, std::max(lane[0], lane[1])); }
-  };
+// Runs and where they go.
+struct Deal {
+  std::vector<Run> runs;
   std::vector<Cta> cta;
-  explicit Dealer(int32_t ctas) : cta(size_t(ctas)) {
-    std::vector<Load> v(cta.size());
-    for (size_t c = 0; c < v.size(); ++c) v[c] = {0, int32_t(c)};
-    free = decltype(free)(std::greater<Load>(), std::move(v));
-  }
-  struct Place {
-    int32_t cta, lane;
-  };
-  Place deal(const Cost& c) {
-    const int32_t at = free.top().second;
-    free.pop();
-    Cta& t = cta[size_t(at)];
-    int32_t lane = 0;
-    if (c.kind == 2) {
-      t.pairs += c.shared;
-    } else {
-      lane = t.lane[1] < t.lane[0] ? 1 : 0;
-      t.lane[lane] += c.chain;
-      t.shared += c.shared;
+  std::vector<std::vector<int32_t>> dealt;  // of each CTA: runs of two Q tiles, of lane 0, of lane 1
+
+  // Hands out runs (indices, longest first) to the CTA that is free first, and those of one Q tile to its lane that is.
+  void hand_out(const std::vector<int32_t>& order) {
+    using Load = std::pair<int64_t, int32_t>;  // (free at, CTA)
+    std::vector<Load> loads(cta.size());
+    for (size_t c = 0; c < cta.size(); ++c) loads[c] = {cta[c].free_at(), int32_t(c)};
+    std::priority_queue<Load, std::vector<Load>, std::greater<Load>> next(std::greater<Load>(), std::move(loads));
+    for (const int32_t i : order) {
+      const Cost& c = runs[size_t(i)].cost;
+      const int32_t at = next.top().second;
+      next.pop();
+      Cta& t = cta[size_t(at)];
+      int32_t list = 0;
+      if (c.kind == 2) {
+        t.pairs += c.shared;
+      } else {
+        const int32_t lane = t.lane[1] < t.lane[0] ? 1 : 0;
+        t.lane[lane] += c.chain;
+        t.shared += c.shared;
+        list = 1 + lane;
+      }
+      dealt[size_t(at) * 3 + size_t(list)].push_back(i);
+      next.push({t.free_at(), at});
     }
-    // by the shared time: a CTA with one busy lane takes a second piece almost for nothing
-    free.push({t.pairs + std::max(t.shared, std::min(t.lane[0], t.lane[1])), at});
-    return {at, lane};
   }
   int64_t end() const {
     int64_t e = 0;
     for (const Cta& t : cta) e = std::max(e, t.end());
     return e;
   }
+  int64_t mean() const {
+    int64_t sum = 0;
+    for (const Run& r : runs) sum += r.cost.shared;
+    return sum / int64_t(cta.size());
+  }
 };
 
-bool longer(const Cost& a, const Cost& b) {
-  if (a.kind != b.kind) return a.kind > b.kind;
-  return a.shared > b.shared;
-}
+struct Planner {
+  const std::vector<Item>& items;
+  int32_t sm_count, group, small_tokens;
+  bool has_prefix;  // every piece leaves a partial result
+  bool by_groups;   // K/V of sixteen heads at a time, where all of it would not stay in L2 (see CausalWalk's groups)
+
+  Cost cost(const Run& r) const { return cost_of(cut_piece(items[size_t(r.item)], r.from, r.len), small_tokens); }
+
+  // Items cut into pieces of at most `len` tiles, not dealt yet.
+  Deal uniform(int32_t len) const {
+    Deal d;
+    d.cta.resize(size_t(sm_count));
+    d.dealt.resize(size_t(sm_count) * 3);
+    for (size_t i = 0; i < items.size(); ++i) {
+      const int32_t longest = items[i].longest(), n = (longest + len - 1) / len, l = (longest + n - 1) / n;
+      for (int32_t from = 0; from < longest; from += l) {
+        Run r{int32_t(i), from, std::min(l, longest - from), {}};
+        r.cost = cost(r);
+        d.runs.push_back(r);
+      }
+    }
+    return d;
+  }
+
+  void deal(Deal* d) const {
+    // by kind, then by group of heads, then longest first
+    std::vector<std::pair<uint64_t, int32_t>> keys(d->runs.size());
+    for (size_t i = 0; i < keys.size(); ++i) {
+      const Run& r = d->runs[i];
+      const uint64_t head_group = by_groups ? uint64_t(items[size_t(r.item)].kv_head / 16) : 0;
+      keys[i] = {(uint64_t(2 - r.cost.kind) << 62) | (head_group << 44) | ((uint64_t(1) << 44) - 1 - uint64_t(r.cost.shared)),
+                 int32_t(i)};
+    }
+    std::sort(keys.begin(), keys.end());
+    std::vector<int32_t> order(keys.size());
+    for (size_t i = 0; i < order.size(); ++i) order[i] = keys[i].second;
+    d->hand_out(order);
+  }
+
+  // Takes from every CTA that ends after `limit` the end of its longest run, and hands that out again.
+  Deal trimmed(const Deal& from, int64_t limit) const {
+    Deal d = from;
+    std::vector<int32_t> loose;
+    for (size_t c = 0; c < d.cta.size(); ++c) {
+      const int64_t excess = d.cta[c].end() - limit;
+      if (excess <= 0 || d.dealt[c * 3].empty()) continue;
+      const size_t at = size_t(d.dealt[c * 3].front());
+      const int32_t tiles = std::max<int32_t>(kShortestCut, int32_t((excess + kTilePair - 1) / kTilePair));
+      if (d.runs[at].len - tiles < kShortestCut) continue;
+      Run rest{d.runs[at].item, d.runs[at].from + d.runs[at].len - tiles, tiles, {}};
+      d.runs[at].len -= tiles;
+      rest.cost = cost(rest);
+      const Cost shorter = cost(d.runs[at]);
+      d.cta[c].pairs -= d.runs[at].cost.shared - shorter.shared;
+      d.runs[at].cost = shorter;
+      loose.push_back(int32_t(d.runs.size()));
+      d.runs.push_back(rest);
+    }
+    std::stable_sort(loose.begin(), loose.end(), [&](int32_t a, int32_t b) {
+      return d.runs[size_t(a)].cost.shared > d.runs[size_t(b)].cost.shared;
+    });
+    d.hand_out(loose);
+    return d;
+  }
+
+  // What the join adds.
+  int64_t join(const Deal& d) const {
+    std::vector<int32_t> runs_of(items.size(), 0);
+    for (const Run& r : d.runs) ++runs_of[size_t(r.item)];
+    int64_t rows = 0;
+    for (const Run& r : d.runs)
+      if (has_prefix || runs_of[size_t(r.item)] > 1) rows += int64_t(items[size_t(r.item)].n_tokens) * group;
+    return rows > 0 ? kJoin + rows / kJoinRows : 0;
+  }
+
+  Deal best() const {
+    int64_t total_tiles = 0, long_items = 0;
+    int32_t longest = 1;
+    bool pairs = false;
+    for (const Item& it : items) {
+      total_tiles += it.longest();
+      longest = std::max(longest, it.longest());
+      pairs = pairs || it.tiles1 > 0;
+    }
+    for (const Item& it : items) long_items += 2 * it.longest() > longest ? 1 : 0;
+    std::vector<int32_t> lens;
+    auto consider = [&](int64_t len) {
+      len = std::max<int64_t>(1, len);
+      if (len < longest && std::find(lens.begin(), lens.end(), int32_t(len)) == lens.end()) lens.push_back(int32_t(len));
+    };
+    const int64_t even = (total_tiles + sm_count - 1) / sm_count;
+    for (const int64_t parts : {1, 2, 4, 8}) consider((even + parts - 1) / parts);
+    consider((longest + 1) / 2);
+    consider((3 * int64_t(longest) + 3) / 4);
+    // as many pieces of the longest items as fill the CTAs, or their lanes, a whole number of times
+    for (const int64_t rounds : {1, 2, 4}) {
+      const int64_t n = long_items > 0 ? rounds * sm_count / long_items : 0;
+      if (n > 1) consider((longest + n - 1) / n);
+    }
+
+    Deal found = uniform(longest);
+    deal(&found);
+    int64_t end = found.end() + join(found);
+    const Deal whole = found;
+    auto offer = [&](Deal&& d) {
+      const int64_t e = d.end() + join(d);
+      if (e >= end) return;
+      end = e;
+      found = std::move(d);
+    };
+    // What a few CTAs have too much. With fewer items than CTAs there is nothing to even out.
+    if (pairs && items.size() > size_t(sm_count))
+      for (const int64_t percent : {101, 102, 104, 107})
+        if (whole.mean() * percent / 100 + kJoin < end) offer(trimmed(whole, whole.mean() * percent / 100 + kPairStart));
+    for (const int32_t len : lens) {
+      Deal d = uniform(len);
+      if (d.mean() + join(d) >= end - end / 100) continue;  // no better to speak of, however it is dealt
+      deal(&d);
+      offer(std::move(d));
+    }
+    return found;
+  }
+};
 
 }  // namespace
 
@@ -149,6 +276,8 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   }
   plan->rows_q = first_token.back();
   if (plan->rows_q >= (int64_t(1) << 31) - 256) return "too many query rows";
+
+  const bool has_prefix = in.len_prefix > 0;
 
   // ---- items
   std::vector<Item> items;
@@ -203,89 +332,38 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
       }
     }
   }
-  const bool has_prefix = in.len_prefix > 0;
-
-  // ---- how long a piece may be
-  int64_t total_tiles = 0;
-  int32_t longest = 0;
-  for (const Item& it : items) {
-    total_tiles += it.longest();
-    longest = std::max(longest, it.longest());
-  }
-  int32_t best_len = std::max(longest, 1);
-  if (!items.empty()) {
-    std::vector<int32_t> lens{std::max(longest, 1)};
-    auto consider = [&](int64_t len) {
-      len = std::max<int64_t>(1, len);
-      if (len < longest && std::find(lens.begin(), lens.end(), int32_t(len)) == lens.end()) lens.push_back(int32_t(len));
-    };
-    const int64_t even = (total_tiles + in.sm_count - 1) / in.sm_count;
-    for (const int64_t parts : {1, 2, 3, 4, 6, 8}) consider((even + parts - 1) / parts);
-    consider((longest + 1) / 2);
-    consider((3 * int64_t(longest) + 3) / 4);
-    // as many pieces of the longest items as fill the CTAs, or their lanes, a whole number of times
-    int64_t long_items = 0;
-    for (const Item& it : items) long_items += 2 * it.longest() > longest ? 1 : 0;
-    for (const int64_t rounds : {1, 2, 3, 4, 6}) {
-      const int64_t n = rounds * in.sm_count / long_items;
-      if (n > 1) consider((longest + n - 1) / n);
-    }
-    int64_t best = -1;
-    std::vector<Cost> costs;
-    for (const int32_t len : lens) {
-      costs.clear();
-      bool any_cut = has_prefix;
-      int64_t rows = 0;
-      for (const Item& it : items) {
-        const int32_t n = cuts_of(it, len), l = even_len(it, len);
-        any_cut = any_cut || n > 1;
-        for (int32_t c = 0; c < n; ++c)
-          costs.push_back(cost_of(cut_piece(it, c * l, std::min(l, it.longest() - c * l)), small_tokens));
-        if (n > 1 || has_prefix) rows += int64_t(n) * it.n_tokens * group;
-      }
-      std::sort(costs.begin(), costs.end(), longer);
-      Dealer dealer(in.sm_count);
-      for (const Cost& c : costs) dealer.deal(c);
-      const int64_t end = dealer.end() + (any_cut ? kJoin + rows / kJoinRows : 0);
-      if (best < 0 || end < best) {
-        best = end;
-        best_len = len;
-      }
-    }
-  }
-
   // ---- pieces, with the rows of their partial results
-  struct Piece {
-    PlanPiece p;
-    Cost cost;
-    int32_t head_group;
-  };
-  // K/V of sixteen heads at a time where all of it would not stay in L2 (see CausalWalk's groups)
   const bool by_groups = kv_bytes > (int64_t(64) << 20);
-  std::vector<Piece> pieces;
+  const Deal deal = Planner{items, in.sm_count, group, small_tokens, has_prefix, by_groups}.best();
+  std::vector<int32_t> by_item(deal.runs.size());  // runs in the order of items and keys
+  for (size_t i = 0; i < by_item.size(); ++i) by_item[i] = int32_t(i);
+  std::sort(by_item.begin(), by_item.end(), [&](int32_t a, int32_t b) {
+    const Run &x = deal.runs[size_t(a)], &y = deal.runs[size_t(b)];
+    return x.item != y.item ? x.item < y.item : x.from < y.from;
+  });
+  std::vector<PlanPiece> pieces(deal.runs.size());  // of each run
   std::vector<int32_t> item_piece0(items.size() + 1, 0);
   int64_t slots = 0;
-  for (size_t i = 0; i < items.size(); ++i) {
-    const Item& it = items[i];
-    item_piece0[i] = int32_t(pieces.size());
-    const int32_t n = cuts_of(it, best_len), l = even_len(it, best_len);
-    for (int32_t c = 0; c < n; ++c) {
-      Piece p{};
-      p.p = cut_piece(it, c * l, std::min(l, it.longest() - c * l));
-      if (n > 1 || has_prefix) {
-        p.p.slot_row = int32_t(slots);
-        slots += int64_t(it.n_tokens) * group;
-        if (slots >= (int64_t(1) << 31) - 512) return "too many partial rows";
-      }
-      p.cost = cost_of(p.p, small_tokens);
-      p.head_group = by_groups ? it.kv_head / 16 : 0;
-      pieces.push_back(p);
+  for (size_t k = 0, i = 0; i < items.size(); ++i) {
+    item_piece0[i] = int32_t(k);
+    size_t last = k;
+    while (last < by_item.size() && deal.runs[size_t(by_item[last])].item == int32_t(i)) ++last;
+    const bool partial = has_prefix || last - k > 1;
+    for (; k < last; ++k) {
+      const Run& r = deal.runs[size_t(by_item[k])];
+      PlanPiece& p = pieces[size_t(by_item[k])];
+      p = cut_piece(items[i], r.from, r.len);
+      if (!partial) continue;
+      p.slot_row = int32_t(slots);
+      slots += int64_t(items[i].n_tokens) * group;
+      if (slots >= (int64_t(1) << 31) - 512) return "too many partial rows";
     }
   }
   item_piece0[items.size()] = int32_t(pieces.size());
   if (pieces.size() >= (size_t(1) << 24)) return "too many pieces";
   plan->slot_rows = slots;
   plan->pieces = int32_t(pieces.size());
+  auto slot_of = [&](int32_t k) { return pieces[size_t(by_item[size_t(k)])].slot_row; };
 
   // ---- join units
   std::vector<PlanUnit> units;
@@ -316,11 +394,11 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
             count = std::min(count, (b + 1) * block - u.token);
             const size_t item = prefix_at + size_t(b) * size_t(heads_kv) + size_t(h);
             for (int32_t p = item_piece0[item]; p < item_piece0[item + 1]; ++p)
-              parts.push_back(pieces[size_t(p)].p.slot_row + (u.token - b * block) * group);
+              parts.push_back(slot_of(p) + (u.token - b * block) * group);
           }
           if (own)
             for (int32_t p = item_piece0[own_item]; p < item_piece0[own_item + 1]; ++p)
-              parts.push_back(pieces[size_t(p)].p.slot_row + i * group);
+              parts.push_back(slot_of(p) + i * group);
           u.n_tokens = count;
           u.parts = int32_t(parts.size()) - u.part0;
           units.push_back(u);
@@ -333,25 +411,10 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
   if (units.size() >= (size_t(1) << 28) || parts.size() >= (size_t(1) << 28)) return "too many rows to join";
   plan->units = int32_t(units.size());
 
-  // ---- dealing: longest first, each to the CTA that is free first
-  std::vector<int32_t> order(pieces.size());
-  for (size_t i = 0; i < order.size(); ++i) order[i] = int32_t(i);
-  std::stable_sort(order.begin(), order.end(), [&](int32_t a, int32_t b) {
-    const Piece &x = pieces[size_t(a)], &y = pieces[size_t(b)];
-    if (x.cost.kind == y.cost.kind && x.head_group != y.head_group) return x.head_group < y.head_group;
-    return longer(x.cost, y.cost);
-  });
-  std::vector<std::vector<int32_t>> dealt(size_t(in.sm_count) * 3);  // pairs, lane 0, lane 1 of each CTA
-  Dealer dealer(in.sm_count);
-  for (const int32_t i : order) {
-    const Cost& c = pieces[size_t(i)].cost;
-    const Dealer::Place at = dealer.deal(c);
-    dealt[size_t(at.cta) * 3 + size_t(c.kind == 2 ? 0 : 1 + at.lane)].push_back(i);
-  }
   plan->grid = 0;
   for (int32_t c = 0; c < in.sm_count; ++c)
     for (int32_t k = 0; k < 3; ++k)
-      if (!dealt[size_t(c) * 3 + size_t(k)].empty()) plan->grid = c + 1;
+      if (!deal.dealt[size_t(c) * 3 + size_t(k)].empty()) plan->grid = c + 1;
 
   // ---- table
   const size_t unit_at = size_t(kPlanPieceAt) + pieces.size() * (sizeof(PlanPiece) / 4);
@@ -369,7 +432,7 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
     for (int32_t part = 0; part < 3; ++part) {
       t[kPlanCtaAt + kPlanCtaWords * c + part] = k;
       if (c < in.sm_count)
-        for (const int32_t i : dealt[size_t(c) * 3 + size_t(part)]) out[k++] = pieces[size_t(i)].p;
+        for (const int32_t i : deal.dealt[size_t(c) * 3 + size_t(part)]) out[k++] = pieces[size_t(i)];
     }
     const int32_t begin = t[kPlanCtaAt + kPlanCtaWords * c];
     t[kPlanCtaAt + kPlanCtaWords * c + 3] = k;
