@@ -24,9 +24,10 @@ constexpr int kTile = 128;
 // A piece of one Q tile runs on one of a CTA's two lanes: alone it is bound by its chain of steps, beside another lane
 // by what the two share, which is above all memory (64 KB per tile).
 constexpr int64_t kTilePair = 1000;
+constexpr int64_t kTilePairPrefix = 1250;  // the same, with every CTA on keys of its own, which come from memory
 constexpr int64_t kPairStart = 2200;    // Q load, first scores, last PV, stores
 constexpr int64_t kTileShared = 930;
-constexpr int64_t kSharedStart = 1000;
+constexpr int64_t kSharedStart = 750;
 constexpr int64_t kTileChain = 950;     // scores, softmax, PV of one tile after the other
 constexpr int64_t kChainStart = 1300;
 constexpr int64_t kJoin = 2500;         // the second kernel, once,
@@ -45,7 +46,7 @@ struct Cost {
   int64_t chain;   // of a lane's time, for one Q tile
 };
 Cost cost_of(const PlanPiece& p, int32_t small_tokens) {
-  if (p.tiles[1] > 0) return {2, kPairStart + p.tiles[1] * kTilePair, 0};
+  if (p.tiles[1] > 0) return {2, kPairStart + p.tiles[1] * (p.source == 1 ? kTilePairPrefix : kTilePair), 0};
   return {p.n_tokens <= small_tokens ? 0 : 1, kSharedStart + p.tiles[0] * kTileShared,
           kChainStart + p.tiles[0] * kTileChain};
 }
