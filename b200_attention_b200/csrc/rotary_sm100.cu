@@ -12,9 +12,8 @@
 // into the cosines and sines once per token and only the row's scale is left to apply per head; arithmetic is on
 // packed pairs of 32-bit values.
 // Measured at 16384 tokens, 32 + 8 heads: half a warp per head with every lane working out its own four angles ran
-// 47.6 M warp instructions and was bound by them (71 us, 4.7 TB/s); this form takes 61.5 us, 5.5 TB/s, 85 % of what a
-// plain copy reaches. Blocks of 4 warps with 2 heads ahead against 8 warps: 63.4 and 65.1 us; 1 head ahead and more
-// warps per SM: 67.5 us.
+// 47.6 M warp instructions and was bound by them (71 us, 4.7 TB/s); this form takes 59.7 us, 5.6 TB/s, 87 % of what a
+// plain copy reaches. Blocks of 4 warps against 8: 63.4 and 65.1 us.
 // Statistics and rotation are in 32 bits and rounded to bf16 once. Angles are reduced to a fraction of a turn in
 // 64 bits first: at position 10^6 a 32-bit product is already off by 0.03 radians.
 
@@ -36,9 +35,15 @@ using ptx::f2_splat;
 using ptx::pack_bf16x2;
 
 constexpr int kWarps = 4;
-constexpr int kBlocksPerSm = 6;  // 85 registers: 24 warps with two heads each on their way hold 48 KB of loads per SM
 constexpr int kPairs = 64;
-constexpr int kDepth = 2;  // heads of a quarter warp that are on their way while one is worked on
+// Two numbers make a variant: the heads of a quarter warp that are on their way while one is worked on, and the blocks
+// per SM that the registers are shared out for. Measured (us):
+//                                               2 ahead, 6 blocks   1 ahead, 7 blocks   1 ahead, 6 blocks
+//   16384 tokens x 40 heads (10 heads a quarter)      59.7                62.0                64.6
+//   65536 tokens x 24 heads (6)                      155.2               147.6               155.7
+//   1537 tokens x 24 heads, 2 warps a token (3)        6.8                 6.9                 6.2
+//   32 tokens x 40 heads, 10 warps a token (1)         4.0                 3.7                 3.6
+constexpr int kFewHeads = 24;  // of a token in one warp
 
 __device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
   f2 r;
@@ -76,7 +81,7 @@ __device__ __forceinline__ float weight_of(const void* w, int is_fp32, int i) {
 
 // Heads h0, h0 + 4, .. < end of one operand for the calling quarter warp (h0 already counts the quarter).
 // `turn` holds (cos, sin) of the token's 64 pairs and is ready once `angles` has been called.
-template <bool kInterleaved, class Angles>
+template <bool kInterleaved, int kDepth, class Angles>
 __device__ __forceinline__ void rotate_heads(const RotaryOperand& x, const RotaryParams& p, int64_t b, int64_t t, int h0,
                                              int end, int l, const float2* turn, const float* w, Angles angles) {
   const char* src = reinterpret_cast<const char*>(x.in + b * x.in_stride_b + t * x.in_stride_t + h0 * x.in_stride_h + 8 * l);
@@ -171,7 +176,7 @@ __device__ __forceinline__ void rotate_heads(const RotaryOperand& x, const Rotar
   }
 }
 
-template <bool kInterleaved>
+template <bool kInterleaved, int kDepth, int kBlocksPerSm>
 __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_norm_rope_kernel(const RotaryParams p) {
   __shared__ alignas(16) float2 turns_of[kWarps][kPairs];
   __shared__ alignas(16) float weights[2][128];  // 1 where there is none
@@ -181,11 +186,13 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_norm_rope_kernel
     weights[i >> 7][i & 127] = weight_of((i >> 7) ? p.k.weight : p.q.weight, p.weight_fp32, i & 127);
   __syncthreads();
   const int lane = threadIdx.x & 31, l = lane & 7, quarter = lane >> 3;
-  const int64_t unit = int64_t(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-  const int64_t row = unit / p.chunks;
-  if (row >= int64_t(p.batch) * p.tokens) return;  // whole warps
-  const int chunk = int(unit - row * p.chunks);
-  const int64_t b = row / p.tokens, t = row - b * p.tokens;
+  // (64-bit divisions here cost as many instructions as two heads; there are fewer than 2^31 tokens, and chunks only
+  // where there are few)
+  const uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const uint32_t row = p.chunks == 1 ? unit : unit / uint32_t(p.chunks);
+  const uint32_t b = p.batch == 1 ? 0 : row / uint32_t(p.tokens), t = row - b * uint32_t(p.tokens);
+  if (b >= uint32_t(p.batch) || t >= uint32_t(p.tokens)) return;  // whole warps
+  const int chunk = int(unit - row * uint32_t(p.chunks));
   float2* turn = turns_of[threadIdx.x >> 5];
 
   bool have = false;
@@ -210,26 +217,34 @@ __global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) qk_norm_rope_kernel
   // a warp's heads: some of q's, or of k's, or the last of q's and the first of k's
   const int first = chunk * p.chunk_heads, end = min(p.heads_q + p.heads_k, first + p.chunk_heads);
   if (first < p.heads_q)
-    rotate_heads<kInterleaved>(p.q, p, b, t, first + quarter, min(end, p.heads_q), l, turn, weights[0], angles);
+    rotate_heads<kInterleaved, kDepth>(p.q, p, b, t, first + quarter, min(end, p.heads_q), l, turn, weights[0], angles);
   if (end > p.heads_q)
-    rotate_heads<kInterleaved>(p.k, p, b, t, max(first, p.heads_q) - p.heads_q + quarter, end - p.heads_q, l, turn, weights[1], angles);
+    rotate_heads<kInterleaved, kDepth>(p.k, p, b, t, max(first, p.heads_q) - p.heads_q + quarter, end - p.heads_q, l, turn, weights[1], angles);
 }
 
 }  // namespace
+
+template <int kDepth, int kBlocksPerSm>
+static cudaError_t launch_variant(const RotaryParams& p, bool interleaved, int64_t rows, cudaStream_t stream) {
+  const int64_t blocks = (rows * p.chunks + kWarps - 1) / kWarps;
+  return launch_overlapped(interleaved ? qk_norm_rope_kernel<true, kDepth, kBlocksPerSm>
+                                       : qk_norm_rope_kernel<false, kDepth, kBlocksPerSm>,
+                           unsigned(blocks), kWarps * 32, 0, stream, p);
+}
 
 cudaError_t launch_qk_norm_rope(RotaryParams p, bool interleaved, int sm_count, cudaStream_t stream) {
   const int64_t rows = int64_t(p.batch) * p.tokens;
   const int heads = p.heads_q + p.heads_k;
   // With few tokens a token's heads are spread over several warps (each works the angles out again), as far as all
   // warps are still resident at once.
-  const int64_t resident = int64_t(sm_count) * kBlocksPerSm * kWarps, most = (heads + 3) / 4;
+  const int64_t resident = int64_t(sm_count) * 6 * kWarps, most = (heads + 3) / 4;
   int chunks = 1;
   if (rows * 2 <= resident) chunks = int(resident / rows < most ? resident / rows : most);
   p.chunk_heads = ((heads + chunks - 1) / chunks + 3) / 4 * 4;
   p.chunks = (heads + p.chunk_heads - 1) / p.chunk_heads;
-  const int64_t blocks = (rows * p.chunks + kWarps - 1) / kWarps;
-  return launch_overlapped(interleaved ? qk_norm_rope_kernel<true> : qk_norm_rope_kernel<false>, unsigned(blocks),
-                           kWarps * 32, 0, stream, p);
+  if (p.chunks > 1) return launch_variant<1, 6>(p, interleaved, rows, stream);
+  if (heads <= kFewHeads) return launch_variant<1, 7>(p, interleaved, rows, stream);
+  return launch_variant<2, 6>(p, interleaved, rows, stream);
 }
 
 }  // namespace b200attn
