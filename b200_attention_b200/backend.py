@@ -135,8 +135,12 @@ class B200Attention:
 
     label = "B200Attention"
 
-    def __init__(self, *, softmax_scale: float = 0.0) -> None:
+    def __init__(self, *, softmax_scale: float = 0.0, qk=None) -> None:
+        """qk: a rotary.QkNormRope (or any callable on [B, T, H, 128] query and key that returns both), applied before
+        attending: norm per head and rotation by position, for models that leave them to the attention callable. Its
+        positions are the tokens' of query and key alike, so it belongs to self-attention."""
         self._softmax_scale = float(softmax_scale)
+        self._qk = qk
         self._loaded = False
 
     def __call__(self, query, key, value, heads: int, mask=None):
@@ -156,6 +160,8 @@ class B200Attention:
             return v if ok else v.contiguous()
 
         q4, k4, v4 = as_bshd(query), as_bshd(key), as_bshd(value)
+        if self._qk is not None:
+            q4, k4 = self._qk(q4, k4)
         out = ops.attention(q4, k4, v4, layout="bshd", softmax_scale=self._softmax_scale)
         output = out.view(batch, lq, heads * head_dim)
         _LOG.add((query, key, value), (batch, lq, lk, heads, head_dim))

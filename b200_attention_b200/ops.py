@@ -4,6 +4,10 @@
 pointers and strides (no copies, any layout whose head_dim axis is dense). The
 `torch.ops.b200_attention_b200.*` ops registered by the C++ shim are reached through
 `registry.load_kernel()`.
+
+Beside it, for serving: `attention_packed()` and `attention_shared_prefix()` (sequences of different
+lengths, whole prompts to single tokens, requests behind a common prefix; packed.py) and
+`qk_norm_rope()` (norm of queries and keys per head and their rotation by position; rotary.py).
 """
 
 from __future__ import annotations
@@ -15,7 +19,7 @@ import torch
 
 from . import _native as N
 from .packed import AttentionPlan, attention_packed, attention_shared_prefix  # noqa: F401
-from .rotary import qk_norm_rope  # noqa: F401
+from .rotary import QkNormRope, qk_norm_rope  # noqa: F401
 
 HEAD_DIM = 128
 

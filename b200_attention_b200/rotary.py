@@ -121,4 +121,19 @@ def _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interl
     return q_out, k_out if k is not None else None
 
 
-__all__ = ["qk_norm_rope"]
+class QkNormRope:
+    """qk_norm_rope with everything but q and k given once: what stands in front of a layer's attention. Accepted by
+    backend.B200Attention, which applies it to query and key before it attends."""
+
+    def __init__(self, positions: torch.Tensor, inv_freq: torch.Tensor, *, sections: Optional[Sequence[int]] = None,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False):
+        self.positions, self.inv_freq = positions, inv_freq
+        self.options = dict(sections=None if sections is None else tuple(sections), q_weight=q_weight, k_weight=k_weight,
+                            eps=eps, interleaved=interleaved)
+
+    def __call__(self, q: torch.Tensor, k: Optional[torch.Tensor], *, out=None, stream=None):
+        return qk_norm_rope(q, k, self.positions, self.inv_freq, out=out, stream=stream, **self.options)
+
+
+__all__ = ["QkNormRope", "qk_norm_rope"]
