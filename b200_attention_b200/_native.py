@@ -249,24 +249,6 @@ def lib() -> C.CDLL:
     return _lib
 
 
-_torch_ops = None
-
-
-def torch_ops():
-    """torch.ops.b200_attention_b200, with libb200attn.so and the torch shim loaded (once); raises if they have not been
-    built."""
-    global _torch_ops
-    if _torch_ops is None:
-        import torch
-
-        lib()
-        if not TORCH_LIB.exists():
-            raise ImportError(f"{TORCH_LIB} is missing: run `python -m b200_attention_b200.build`")
-        torch.ops.load_library(str(TORCH_LIB))
-        _torch_ops = torch.ops.b200_attention_b200
-    return _torch_ops
-
-
 _direct = None
 
 

@@ -22,7 +22,8 @@ constexpr int kStatusInts = 8;
 enum DeviceCode : int32_t {
   kDevOk = 0,
   kDevWaitTimeout = 1,    // a bounded mbarrier wait ran out
-  kDevSmemMisaligned = 2  // dynamic shared memory base was not 1024-byte aligned
+  kDevSmemMisaligned = 2, // dynamic shared memory base was not 1024-byte aligned
+  kDevNoPlan = 3          // a planned call found something else where its table should be
 };
 
 // Chaining calls over successive K/V shards (the sequence-parallel ring): every call

@@ -660,7 +660,13 @@ __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t ba
       }
       tc_fence_before_sync();
       __syncwarp();
+#ifdef B200ATTN_TEST_DROP_P_READY
+      // Test builds only (never the shipped library): see attn_fwd_ws_kernel.
+      const bool withheld = (q == 0 && warp_in_group == 0 && n == 0 && i == 1);
+      mbar_arrive_lead((lane == 0 && !withheld) ? 1u : 0u, bar(kPbPReady + q));
+#else
       mbar_arrive_lead(lane == 0 ? 1u : 0u, bar(kPbPReady + q));
+#endif
     }
     const Pieces ps(p, aux);
     if (n != ps.last_of(q)) {
@@ -752,10 +758,11 @@ attn_plan_kernel(const __grid_constant__ PlanMaps maps, const PlanParams p) {
   if (warp == 13 && lane < 6) tma_prefetch_desc(&maps.q + lane);
   const int4 first = record[0];
   const int piece0 = first.x, piece1 = first.w;
-  if (misaligned || piece0 >= piece1) {  // uniform across the CTA; the latter: a table with fewer CTAs than the grid
-    if (threadIdx.x == 0 && misaligned) {
+  const bool no_plan = p.table[kPlanHdrMagic] != kPlanMagic;  // freed memory, say, under a captured call
+  if (misaligned || no_plan || piece0 >= piece1) {  // uniform across the CTA; the last: fewer CTAs than the grid
+    if (threadIdx.x == 0 && (misaligned || no_plan)) {
       aux->abort_flag = 0;
-      w.raise(kDevSmemMisaligned, 3, 0);
+      w.raise(misaligned ? kDevSmemMisaligned : kDevNoPlan, 3, 0);
     }
     wait_for_previous();
     return;
@@ -925,7 +932,7 @@ attn_plan_join_kernel(const PlanParams p) {
   __shared__ float4 shared_acc[kJoinWarps][32];
   __shared__ float shared_m[kJoinWarps], shared_sum[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int units = p.table[kPlanHdrUnits];
+  const int units = p.table[kPlanHdrMagic] == kPlanMagic ? p.table[kPlanHdrUnits] : 0;
   const PlanUnit* unit = reinterpret_cast<const PlanUnit*>(p.table + p.table[kPlanHdrUnitAt]);
   const int32_t* part_list = p.table + p.table[kPlanHdrPartAt];
   // (This kernel does not let the next one be brought up before its own end: with 512 units that left the next call's

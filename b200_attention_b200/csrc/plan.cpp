@@ -32,6 +32,8 @@ constexpr int64_t kTileChain = 950;     // scores, softmax, PV of one tile after
 constexpr int64_t kChainStart = 1300;
 constexpr int64_t kJoin = 2500;         // the second kernel, once,
 constexpr int64_t kJoinRows = 14;       // and per row of partial results, divided by this
+// A piece is walked without a look at the other CTAs, under waits of limited length: keep it below a tenth of a second.
+constexpr int32_t kLongestPiece = 1 << 15;
 constexpr int32_t kShortestCut = 3;     // tiles of what is left, and of what is taken, where an item is trimmed
 
 struct Item {
@@ -152,7 +154,7 @@ struct Planner {
     std::vector<std::pair<uint64_t, int32_t>> keys(d->runs.size());
     for (size_t i = 0; i < keys.size(); ++i) {
       const Run& r = d->runs[i];
-      const uint64_t head_group = by_groups ? uint64_t(items[size_t(r.item)].kv_head / 16) : 0;
+      const uint64_t head_group = by_groups ? uint64_t(items[size_t(r.item)].kv_head / 16) & 0x3ffffu : 0;
       keys[i] = {(uint64_t(2 - r.cost.kind) << 62) | (head_group << 44) | ((uint64_t(1) << 44) - 1 - uint64_t(r.cost.shared)),
                  int32_t(i)};
     }
@@ -223,6 +225,7 @@ struct Planner {
       if (n > 1) consider((longest + n - 1) / n);
     }
 
+    longest = std::min(longest, kLongestPiece);
     Deal found = uniform(longest);
     deal(&found);
     int64_t end = found.end() + join(found);

@@ -1,5 +1,5 @@
 // Tensor-level bodies of the packed, shared-prefix and norm-and-rotation calls: argument rules, outputs, workspace, launch.
-// Behind the torch ops (torch_ops.cpp) and behind b200_attention_b200.packed and .rotary (direct.cpp).
+// Behind b200_attention_b200.packed and .rotary (direct.cpp).
 #pragma once
 
 #include <ATen/ATen.h>

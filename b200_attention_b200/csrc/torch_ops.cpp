@@ -15,13 +15,13 @@
 #include <tuple>
 
 #include "../../include/b200_attention.h"
-#include "serving_calls.h"
 
 namespace {
 
-using b200attn_torch::attention_planned;
-using b200attn_torch::check_rc;
-using b200attn_torch::qk_norm_rope;
+void check_rc(int rc) {
+  TORCH_CHECK(rc == B200ATTN_OK, "b200attn: ", b200attn_status_string(rc), ": ",
+              b200attn_last_error());
+}
 
 void check_common(const at::Tensor& Q, const at::Tensor& K, const at::Tensor& V) {
   TORCH_CHECK(Q.is_cuda() && K.is_cuda() && V.is_cuda(), "Q, K, V must be CUDA tensors");
@@ -139,11 +139,5 @@ TORCH_LIBRARY(b200_attention_b200, m) {
   m.def("sdpa_lse(Tensor Q, Tensor K, Tensor V, float scale, bool bshd, int kernel) -> (Tensor, Tensor)",
         &sdpa_lse);
   m.def("sdpa_causal_gqa(Tensor Q, Tensor K, Tensor V, float scale) -> (Tensor, Tensor)", &sdpa_causal_gqa);
-  m.def("attention_planned(Tensor q, Tensor k, Tensor v, Tensor? k_prefix, Tensor? v_prefix, Tensor table, int[] plan, "
-        "float scale, bool return_lse, Tensor? out) -> (Tensor, Tensor)",
-        &attention_planned);
-  m.def("qk_norm_rope(Tensor q, Tensor? k, Tensor positions, Tensor inv_freq, int[] sections, Tensor? q_weight, "
-        "Tensor? k_weight, float eps, bool interleaved, Tensor? q_out, Tensor? k_out) -> (Tensor, Tensor)",
-        &qk_norm_rope);
   m.def("device_check() -> ()", &device_check);
 }

@@ -79,6 +79,10 @@ class Schedule:
             lib.b200attn_plan_destroy(handle)
 
 
+# Tables that captured calls read: a graph does not keep the plan alive, and may be replayed without it.
+_tables_of_graphs: list = []
+
+
 class AttentionPlan:
     """Which CTA works on what, for sequences of the given lengths.
 
@@ -90,8 +94,9 @@ class AttentionPlan:
 
     `update` puts other lengths in place. Calls captured into a CUDA graph read the plan's table when the graph is
     replayed, so an updated plan changes what the replay does; `update` refuses lengths that a captured call has no
-    room for. A plan may be used on any stream of its device, also by overlapping calls; only `update` must not overlap
-    calls that use it on other streams than the current one.
+    room for. (What a replay does not compute, rows behind the new last sequence, keeps what the output held.) A plan
+    may be used on any stream of its device, also by overlapping calls; only `update` must not overlap calls that use
+    it on other streams than the current one.
     """
 
     def __init__(self, lens_q, lens_kv, *, heads: int, heads_kv: Optional[int] = None, causal: bool = True,
@@ -101,6 +106,8 @@ class AttentionPlan:
         device = torch.device("cuda" if device is None else device)
         if device.type != "cuda":
             raise RuntimeError("a plan needs a CUDA device (this library has no CPU path)")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a plan cannot be made while the current stream is being captured")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         if torch.cuda.get_device_properties(device).multi_processor_count != 148:
@@ -132,6 +139,8 @@ class AttentionPlan:
         return (*self._now[:5], grid, self._room_units, self._room_slots)
 
     def _hold(self, rows_q: int, rows_kv: int) -> None:
+        if self._captured is None:
+            _tables_of_graphs.append(self._table)
         held = self._captured or (rows_q, rows_kv)
         self._captured = (min(held[0], rows_q), min(held[1], rows_kv))
 
@@ -157,7 +166,12 @@ class AttentionPlan:
 
 def _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream):
     if stream is not None and stream != torch.cuda.current_stream(plan.device):
+        if stream.device != plan.device:
+            raise RuntimeError(f"stream is on {stream.device}, the plan on {plan.device}")
         with torch.cuda.stream(stream):
+            return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
+    if torch.cuda.current_device() != plan.device.index:
+        with torch.cuda.device(plan.device):
             return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
     # a replay may find the table of other lengths: a captured call launches for all that may be in it
     capturing = torch.cuda.is_current_stream_capturing()

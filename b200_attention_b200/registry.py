@@ -75,8 +75,8 @@ def sha256_file(path: Path) -> str:
 def source_closure_sha256(spec: KernelSpec) -> str:
     """Fingerprint of the kernel source and every header it includes (cf. registry.py:230-255)."""
     h = hashlib.sha256()
-    names = ["csrc/attn_fwd_sm100.cu", "csrc/capi.cu", "csrc/noalloc.cu", "csrc/attn_device_sm100.cuh", "csrc/attn_kernels.cuh",
-             "csrc/ptx_sm100.cuh", "csrc/host_common.cuh", "../include/b200_attention.h"]
+    names = ["csrc/attn_fwd_sm100.cu", "csrc/capi.cu", "csrc/noalloc.cu", "csrc/attn_device_sm100.cuh",
+             "csrc/attn_kernels.cuh", "csrc/ptx_sm100.cuh", "csrc/host_common.cuh", "../include/b200_attention.h"]
     for name in names:
         p = (PKG / name).resolve()
         h.update(name.encode())
@@ -102,6 +102,18 @@ class _KernelModule:
         self._ns.device_check()
 
 
+_loaded = False
+
+
 def load_kernel(spec: KernelSpec) -> _KernelModule:
     """Loads libb200attn.so and the torch shim (once) and returns the module-like wrapper."""
-    return _KernelModule(spec, _native.torch_ops())
+    global _loaded
+    import torch
+
+    _native.lib()  # raises if the core library has not been built
+    if not _loaded:
+        if not _native.TORCH_LIB.exists():
+            raise ImportError(f"{_native.TORCH_LIB} is missing: run `python -m b200_attention_b200.build`")
+        torch.ops.load_library(str(_native.TORCH_LIB))
+        _loaded = True
+    return _KernelModule(spec, torch.ops.b200_attention_b200)

@@ -108,6 +108,8 @@ def qk_norm_rope(
         q_out, k_out = out
         _check_out(q, k, q_out, k_out)
     if stream is not None and stream != torch.cuda.current_stream(q.device):
+        if stream.device != q.device:
+            raise RuntimeError(f"stream is on {stream.device}, q on {q.device}")
         with torch.cuda.stream(stream):
             return _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out)
     return _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out)

@@ -288,6 +288,43 @@ def test_two_graphs_of_one_plan_overlap(ops):
     del graphs
 
 
+def test_a_graph_outlives_its_plan(ops):
+    """The table that a captured call reads stays, and so does the memory that its replays need."""
+    import gc
+
+    lens_q, lens_kv = [1, 40], [3000, 40]
+    q, k, v, _, _ = make(lens_q, lens_kv, 8, 2)
+    plan = ops.AttentionPlan(lens_q, lens_kv, heads=8, heads_kv=2)
+    want = ops.attention_packed(q, k, v, plan)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.attention_packed(q, k, v, plan)
+    del plan
+    gc.collect()
+    torch.cuda.empty_cache()
+    noise = [torch.full((n,), -1, dtype=torch.int32, device="cuda") for n in (1000, 20000, 30000, 100000)]
+    graph.replay()
+    settle()
+    assert torch.equal(got, want)
+    del graph, noise
+
+
+def test_plans_and_updates_are_refused_in_a_capture(ops):
+    plan = ops.AttentionPlan([1], [5], heads=2)
+    x = torch.zeros(1, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x += 1
+        with pytest.raises(RuntimeError, match="captured"):
+            ops.AttentionPlan([1], [5], heads=2)
+        with pytest.raises(RuntimeError, match="captured"):
+            plan.update([1], [6])
+    graph.replay()
+    settle()
+    assert x.item() == 1
+    del graph
+
+
 def test_update_in_eager_use(ops):
     plan = ops.AttentionPlan([1], [5], heads=2)
     for lens_q, lens_kv in [([1], [700]), ([300, 2], [300, 9]), ([1] * 50, [4000] * 50)]:
