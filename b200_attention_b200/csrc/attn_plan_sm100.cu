@@ -540,15 +540,24 @@ __device__ __forceinline__ void store_result(const PlanParams& p, const PlanPiec
 #pragma unroll
         for (int j = 0; j < kChunk; ++j) v[j] = seen ? __uint_as_float(acc[u][j]) * weight : 0.0f;
         if (slot_row >= 0) {
-          float4* dst = reinterpret_cast<float4*>(part + (c + u) * kChunk);
+          char* dst = reinterpret_cast<char*>(part + (c + u) * kChunk);
 #pragma unroll
-          for (int j = 0; j < kChunk / 4; ++j) dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          for (int j = 0; j < kChunk; j += 8)
+            st_global_32b(dst + 4 * j, make_uint4(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), __float_as_uint(v[j + 2]), __float_as_uint(v[j + 3])),
+                          make_uint4(__float_as_uint(v[j + 4]), __float_as_uint(v[j + 5]), __float_as_uint(v[j + 6]), __float_as_uint(v[j + 7])));
         } else {
           uint4* dst = reinterpret_cast<uint4*>(out + (c + u) * kChunk);
+          uint4 w[kChunk / 8];
 #pragma unroll
           for (int j = 0; j < kChunk / 8; ++j)
-            dst[j] = make_uint4(pack_bf16x2(v[8 * j + 0], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
-                                pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+            w[j] = make_uint4(pack_bf16x2(v[8 * j + 0], v[8 * j + 1]), pack_bf16x2(v[8 * j + 2], v[8 * j + 3]),
+                              pack_bf16x2(v[8 * j + 4], v[8 * j + 5]), pack_bf16x2(v[8 * j + 6], v[8 * j + 7]));
+          if (p.o_aligned) {
+            st_global_32b(dst, w[0], w[1]);
+          } else {
+            dst[0] = w[0];
+            dst[1] = w[1];
+          }
         }
       }
     }

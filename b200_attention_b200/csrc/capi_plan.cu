@@ -120,8 +120,8 @@ int b200attn_forward_planned(const b200attn_planned_args* a) {
     return fail(B200ATTN_ERR_INVALID_ARGUMENT, "there are no keys to work on");
   if (a->table == nullptr || (reinterpret_cast<uintptr_t>(a->table) & 15u) != 0)
     return fail(B200ATTN_ERR_INVALID_ARGUMENT, "table must be given, 16-byte aligned");
-  if (a->slot_rows < 0 || (a->slot_rows > 0 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 15u) != 0)))
-    return fail(B200ATTN_ERR_INVALID_ARGUMENT, "workspace must be given for slot_rows > 0, 16-byte aligned");
+  if (a->slot_rows < 0 || (a->slot_rows > 0 && (a->workspace == nullptr || (reinterpret_cast<uintptr_t>(a->workspace) & 31u) != 0)))
+    return fail(B200ATTN_ERR_INVALID_ARGUMENT, "workspace must be given for slot_rows > 0, 32-byte aligned");
   if (a->lse != nullptr && a->lse_stride_head < a->rows_q && a->heads > 1)
     return fail(B200ATTN_ERR_INVALID_ARGUMENT, "lse_stride_head must be at least rows_q");
   if (!std::isfinite(a->softmax_scale)) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "softmax_scale must be finite");
@@ -153,6 +153,7 @@ int b200attn_forward_planned(const b200attn_planned_args* a) {
   p.lse_stride_h = a->lse_stride_head;
   p.part_o = static_cast<float*>(a->workspace);
   p.part_lse = p.part_o == nullptr ? nullptr : p.part_o + a->slot_rows * kHeadDim;
+  p.o_aligned = reinterpret_cast<uintptr_t>(o.ptr) % 32 == 0 && o.stride_row % 16 == 0 && o.stride_head % 16 == 0;
   p.group = group;
   p.tile_tokens = plan_tile_tokens(group);
   p.tile_rows = p.tile_tokens * group;

@@ -19,6 +19,7 @@ struct PlanParams {
   int64_t o_stride_t, o_stride_h, lse_stride_h;
   float* part_o;    // [slot rows][128] fp32, normalised
   float* part_lse;  // [slot rows], natural log, -inf where no key was visible
+  int32_t o_aligned;    // every row of o begins on a multiple of 32 bytes
   int32_t group;        // query heads per K/V head
   int32_t tile_tokens;  // floor(128 / group)
   int32_t tile_rows;    // tile_tokens * group

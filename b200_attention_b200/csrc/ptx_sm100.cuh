@@ -320,6 +320,13 @@ __device__ __forceinline__ f2 f2_add(f2 a, f2 b) {
   return r;
 }
 
+// 32 bytes in one store; the address must be 32-byte aligned.
+__device__ __forceinline__ void st_global_32b(void* p, const uint4& a, const uint4& b) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z),
+               "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+               : "memory");
+}
+
 // Two bf16 in one 32-bit word: `lo` in bits 0..15, `hi` in bits 16..31.
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   uint32_t r;

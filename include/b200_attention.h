@@ -243,7 +243,7 @@ typedef struct b200attn_planned_args {
   float softmax_scale;     /* <= 0 selects 1/sqrt(head_dim) */
   int32_t reserved2;       /* 0 */
   const void* table;       /* device memory, 16-byte aligned */
-  void* workspace;         /* device memory, 16-byte aligned, slot_rows * 516 bytes, any contents; calls
+  void* workspace;         /* device memory, 32-byte aligned, slot_rows * 516 bytes, any contents; calls
                             * that may overlap need workspaces of their own */
   int64_t slot_rows;       /* rows the workspace has room for, at least info.slot_rows */
   void* stream;

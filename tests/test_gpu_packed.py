@@ -163,11 +163,14 @@ def test_strided_operands(ops):
     want = ops.attention_packed(q.contiguous(), k.contiguous(), v.contiguous(), plan)
     wide = torch.full((181, 10, 256), 7.0, device="cuda", dtype=torch.bfloat16)
     got = ops.attention_packed(q, k, v, plan, out=wide[:, 1:9, :128])
+    odd = torch.full((181, 8, 136), 7.0, device="cuda", dtype=torch.bfloat16)  # rows on multiples of 16 bytes, not of 32
+    ops.attention_packed(q, k, v, plan, out=odd[:, :, 8:])
     by_head = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
     other = ops.attention_packed(*by_head, plan)
     settle()
     R.check_attention(want, None, R.attention(q, k, v, lens_q, lens_kv, causal=True))
     assert torch.equal(got, want) and torch.equal(other, want)
+    assert torch.equal(odd[:, :, 8:], want) and (odd[:, :, :8] == 7).all()
     assert (wide[:, 0] == 7).all() and (wide[:, 9] == 7).all() and (wide[:, :, 128:] == 7).all()
 
 

@@ -220,7 +220,7 @@ def planned_args(**over):
     (dict(table=0), N.STATUS_INVALID_ARGUMENT),
     (dict(table=0x10008), N.STATUS_INVALID_ARGUMENT),
     (dict(slot_rows=4), N.STATUS_INVALID_ARGUMENT),                          # no workspace
-    (dict(slot_rows=4, workspace=0x10004), N.STATUS_INVALID_ARGUMENT),
+    (dict(slot_rows=4, workspace=0x10010), N.STATUS_INVALID_ARGUMENT),
     (dict(lse=0x10000, lse_stride_head=7), N.STATUS_INVALID_ARGUMENT),
     (dict(softmax_scale=float("inf")), N.STATUS_INVALID_ARGUMENT),
     (dict(q=N.Operand(0, 0, 128, 512)), N.STATUS_INVALID_ARGUMENT),
