@@ -198,9 +198,10 @@ struct Loader {
   __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8u * uint32_t(i); }
 
   // V tile of one piece (or none) and K tile of one (or none) to the next slot of the ring.
+  template <bool kFresh = false>  // on barriers that nobody has used yet
   __device__ __forceinline__ bool push_pair(const PlanPiece* v_pc, int v_tile, const PlanPiece* k_pc, int k_tile, int site,
                                             const WaitCtx& w) {
-    if (!w.wait_issue(bar(kPbPairEmpty + slot), empty_parity, site)) return false;
+    if (!kFresh && !w.wait_issue(bar(kPbPairEmpty + slot), empty_parity, site)) return false;
     const uint32_t full_parity = empty_parity ^ 1u;
     armed |= 1u << slot;
     armed_parity = (armed_parity & ~(1u << slot)) | (full_parity << slot);
@@ -226,12 +227,13 @@ struct Loader {
 
   // Q tile `tile` of a piece to a lane: a box of 64 columns x group heads x tokens lands as rows
   // token * group + head.
+  template <bool kFresh = false>
   __device__ __forceinline__ bool load_q(const PlanPiece* pc, int lane, int tile, const WaitCtx& w) {
     const bool small = is_small(p, pc);
     uint32_t n = 0;  // slot
     if (small) n = (lane ? small_loaded[1]++ : small_loaded[0]++) % kQSlots;
     const int s = lane * kQSlots + int(n);
-    if (!w.wait_issue(bar(kPbQEmpty + s), (q_empty_parity >> s) & 1u, 100 + s)) return false;
+    if (!kFresh && !w.wait_issue(bar(kPbQEmpty + s), (q_empty_parity >> s) & 1u, 100 + s)) return false;
     q_empty_parity ^= 1u << s;
     armed |= 1u << (kPairSlotsP + s);
     armed_parity = (armed_parity & ~(1u << (kPairSlotsP + s))) | (((q_empty_parity >> s) & 1u) << (kPairSlotsP + s));
@@ -244,11 +246,11 @@ struct Loader {
     return true;
   }
 
-  // Q and the first K tile (which travels alone) of the CTA's first piece; on barriers that nobody has used yet.
+  // Q and the first K tile (which travels alone) of the CTA's first piece.
   __device__ __forceinline__ void begin(const PlanPiece* pc, const WaitCtx& w) {
-    load_q(pc, 0, 0, w);
-    push_pair(nullptr, 0, pc, 0, 110, w);
-    if (pc->tiles[1] > 0) load_q(pc, 1, 1, w);
+    load_q<true>(pc, 0, 0, w);
+    push_pair<true>(nullptr, 0, pc, 0, 110, w);
+    if (pc->tiles[1] > 0) load_q<true>(pc, 1, 1, w);
   }
 
   __device__ void run(const PlanAux* aux, WaitCtx& w) {

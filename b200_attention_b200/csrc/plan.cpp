@@ -236,10 +236,13 @@ struct Planner {
       end = e;
       found = std::move(d);
     };
+    // Close to what no schedule can beat: not worth the time of looking for another (a decode step plans anew each time).
+    if (!pairs && end <= whole.mean() * 107 / 100) return found;
     // What a few CTAs have too much. With fewer items than CTAs there is nothing to even out.
     if (pairs && items.size() > size_t(sm_count))
       for (const int64_t percent : {101, 102, 104, 107})
         if (whole.mean() * percent / 100 + kJoin < end) offer(trimmed(whole, whole.mean() * percent / 100 + kPairStart));
+    if (end <= whole.mean() * 104 / 100) return found;
     for (const int32_t len : lens) {
       Deal d = uniform(len);
       if (d.mean() + join(d) >= end - end / 100) continue;  // no better to speak of, however it is dealt
