@@ -40,23 +40,25 @@ bool truth(PyObject* o) {
   return v != 0;
 }
 
-c10::SmallVector<int64_t, 8> integers(PyObject* o, const char* name) {
+c10::SmallVector<int64_t, 12> integers(PyObject* o, const char* name) {
   TORCH_CHECK_TYPE(PyTuple_Check(o), name, " must be a tuple");
-  c10::SmallVector<int64_t, 8> out;
+  c10::SmallVector<int64_t, 12> out;
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(o); ++i) out.push_back(integer(PyTuple_GET_ITEM(o, i)));
   return out;
 }
 
-PyObject* pair_of(const std::tuple<at::Tensor, at::Tensor>& r) {
-  PyObject* out = PyTuple_New(2);
+// A tuple of two tensors (None for an undefined one) and, where `flag` is given, a truth value.
+PyObject* tuple_of(const at::Tensor& a, const at::Tensor& b, const bool* flag = nullptr) {
+  PyObject* out = PyTuple_New(flag != nullptr ? 3 : 2);
   if (out == nullptr) throw python_error();
-  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::get<0>(r)));
-  if (std::get<1>(r).defined()) {
-    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::get<1>(r)));
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(a));
+  if (b.defined()) {
+    PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(b));
   } else {
     Py_INCREF(Py_None);
     PyTuple_SET_ITEM(out, 1, Py_None);
   }
+  if (flag != nullptr) PyTuple_SET_ITEM(out, 2, PyBool_FromLong(*flag ? 1 : 0));
   return out;
 }
 
@@ -64,10 +66,11 @@ PyObject* pair_of(const std::tuple<at::Tensor, at::Tensor>& r) {
 PyObject* attention_planned(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(n == 10, "attention_planned takes 10 arguments");
-  return pair_of(b200attn_torch::attention_planned(tensor(a[0], "q"), tensor(a[1], "k"), tensor(a[2], "v"),
-                                                   maybe_tensor(a[3], "k_prefix"), maybe_tensor(a[4], "v_prefix"),
-                                                   tensor(a[5], "table"), integers(a[6], "plan"), real(a[7]), truth(a[8]),
-                                                   maybe_tensor(a[9], "out")));
+  const auto [o, lse, captured] = b200attn_torch::attention_planned(
+      tensor(a[0], "q"), tensor(a[1], "k"), tensor(a[2], "v"), maybe_tensor(a[3], "k_prefix"),
+      maybe_tensor(a[4], "v_prefix"), tensor(a[5], "table"), integers(a[6], "plan"), real(a[7]), truth(a[8]),
+      maybe_tensor(a[9], "out"));
+  return tuple_of(o, lse, &captured);
   END_HANDLE_TH_ERRORS
 }
 
@@ -75,10 +78,11 @@ PyObject* attention_planned(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   TORCH_CHECK_TYPE(n == 11, "qk_norm_rope takes 11 arguments");
-  return pair_of(b200attn_torch::qk_norm_rope(
+  const auto [qo, ko] = b200attn_torch::qk_norm_rope(
       tensor(a[0], "q"), maybe_tensor(a[1], "k"), tensor(a[2], "positions"), tensor(a[3], "inv_freq"),
       integers(a[4], "sections"), maybe_tensor(a[5], "q_weight"), maybe_tensor(a[6], "k_weight"), real(a[7]), truth(a[8]),
-      maybe_tensor(a[9], "out of q"), maybe_tensor(a[10], "out of k")));
+      maybe_tensor(a[9], "out of q"), maybe_tensor(a[10], "out of k"));
+  return tuple_of(qo, ko);
   END_HANDLE_TH_ERRORS
 }
 

@@ -3,7 +3,9 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -38,15 +40,28 @@ inline void check_rows(const char* name, const at::Tensor& t, int64_t heads, con
 
 inline b200attn_operand row_operand(const at::Tensor& t) { return {t.data_ptr(), 0, t.stride(1), t.stride(0)}; }
 
-// plan: heads, heads_kv, rows_q, rows_kv, len_prefix, grid, join units, slot rows
-inline std::tuple<at::Tensor, at::Tensor> attention_planned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+// What a plan says to a call: heads, heads_kv, rows_q, rows_kv, len_prefix, grid, join units, slot rows; then grid, join
+// units and slot rows for a call that is being captured, whose replays may find the table of other lengths.
+constexpr size_t kPlanInts = 11;
+
+inline at::Tensor empty_on(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
+  return at::detail::empty_cuda(sizes, type, device, std::nullopt);
+}
+
+inline bool capturing(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &status));
+  return status != cudaStreamCaptureStatusNone;
+}
+
+// Returns O, LSE (or an undefined tensor), and whether the call was captured.
+inline std::tuple<at::Tensor, at::Tensor, bool> attention_planned(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                                      const std::optional<at::Tensor>& k_prefix,
                                                      const std::optional<at::Tensor>& v_prefix, const at::Tensor& table,
                                                      at::IntArrayRef plan, double scale, bool return_lse,
                                                      const std::optional<at::Tensor>& out) {
-  TORCH_CHECK(plan.size() == 8, "malformed plan");
+  TORCH_CHECK(plan.size() == kPlanInts, "malformed plan");
   const int64_t heads = plan[0], heads_kv = plan[1], rows_q = plan[2], rows_kv = plan[3], len_prefix = plan[4];
-  const int64_t slots = plan[7];
   const at::Device device = table.device();
   check_rows("q", q, heads, device);
   check_rows("k", k, heads_kv, device);
@@ -69,18 +84,23 @@ inline std::tuple<at::Tensor, at::Tensor> attention_planned(const at::Tensor& q,
   }
 
   c10::cuda::CUDAGuard guard(device);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  const bool captured = capturing(stream);
+  int64_t grid = plan[captured ? 8 : 5];
+  const int64_t units = plan[captured ? 9 : 6], slots = plan[captured ? 10 : 7];
+  if (k.size(0) == 0 && len_prefix == 0) grid = 0;  // no key for any replay to work on
   const int64_t rows = q.size(0);
-  at::Tensor o = out.has_value() ? *out : at::empty({rows, heads, 128}, q.options());
+  at::Tensor o = out.has_value() ? *out : empty_on({rows, heads, 128}, at::kBFloat16, device);
   at::Tensor lse;
-  if (return_lse) lse = at::empty({heads, rows}, q.options().dtype(at::kFloat));
+  if (return_lse) lse = empty_on({heads, rows}, at::kFloat, device);
   if (rows > rows_q) {
     if (!out.has_value()) o.narrow(0, rows_q, rows - rows_q).zero_();
     if (return_lse) lse.narrow(1, rows_q, rows - rows_q).fill_(-std::numeric_limits<float>::infinity());
   }
-  if (rows == 0 || (plan[5] == 0 && plan[6] == 0)) return {o, lse};
+  if (rows == 0 || (grid == 0 && units == 0)) return {o, lse, captured};
   // From the caching allocator at every call: in stream order, and private to a graph that is being captured.
   at::Tensor workspace;
-  if (slots > 0) workspace = at::empty({slots * 129}, q.options().dtype(at::kFloat));
+  if (slots > 0) workspace = empty_on({slots * 129}, at::kFloat, device);
   b200attn_planned_args a{};
   a.struct_bytes = sizeof a;
   a.heads = int32_t(heads);
@@ -89,8 +109,8 @@ inline std::tuple<at::Tensor, at::Tensor> attention_planned(const at::Tensor& q,
   a.rows_q = int32_t(rows);
   a.rows_kv = int32_t(k.size(0));
   a.len_prefix = int32_t(len_prefix);
-  a.grid = int32_t(plan[5]);
-  a.join_units = int32_t(plan[6]);
+  a.grid = int32_t(grid);
+  a.join_units = int32_t(units);
   a.q = row_operand(q);
   a.k = row_operand(k);
   a.v = row_operand(v);
@@ -107,9 +127,9 @@ inline std::tuple<at::Tensor, at::Tensor> attention_planned(const at::Tensor& q,
   a.table = table.data_ptr();
   a.workspace = slots > 0 ? workspace.data_ptr() : nullptr;
   a.slot_rows = slots;
-  a.stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
+  a.stream = stream;
   check_rc(b200attn_forward_planned(&a));
-  return {o, lse};
+  return {o, lse, captured};
 }
 
 inline void check_tokens(const char* name, const at::Tensor& t, const at::Tensor* like) {
@@ -136,6 +156,16 @@ inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, cons
                                                 const std::optional<at::Tensor>& k_weight, double eps, bool interleaved,
                                                 const std::optional<at::Tensor>& q_out,
                                                 const std::optional<at::Tensor>& k_out) {
+  const int64_t axes = int64_t(sections.size());
+  int64_t pairs = 0;
+  for (const int64_t n : sections) {
+    TORCH_CHECK_VALUE(n >= 0 && n <= 64, "sections must be counts of 0 .. 64 pairs");
+    pairs += n;
+  }
+  TORCH_CHECK_VALUE(axes >= 1 && axes <= 4 && pairs >= 1 && pairs <= 64,
+                    "sections must be 1 to 4 counts that add up to 1 .. 64, got ", sections);
+  TORCH_CHECK_VALUE(inv_freq.numel() == pairs, "inv_freq holds ", inv_freq.numel(), " frequencies, sections add up to ",
+                    pairs);
   check_tokens("q", q, nullptr);
   if (k.has_value()) check_tokens("k", *k, &q);
   TORCH_CHECK(k.has_value() || !k_weight.has_value(), "k_weight is given without k");
@@ -147,7 +177,6 @@ inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, cons
   TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong ||
                   positions.scalar_type() == at::kFloat,
               "positions must be int32, int64 or float32, got ", positions.scalar_type());
-  const int64_t axes = int64_t(sections.size());
   const at::Tensor pos = positions.dim() == 1 ? positions.unsqueeze(0) : positions;
   TORCH_CHECK((pos.dim() == 2 && pos.size(0) == axes && pos.size(1) == tokens) ||
                   (pos.dim() == 3 && pos.size(0) == axes && pos.size(1) == batch && pos.size(2) == tokens),
@@ -177,13 +206,12 @@ inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, cons
   }
 
   c10::cuda::CUDAGuard guard(q.device());
-  const at::Tensor qo = given[0] != nullptr ? *given[0] : at::empty(q.sizes(), q.options());
+  const at::Tensor qo = given[0] != nullptr ? *given[0] : empty_on(q.sizes(), at::kBFloat16, q.device());
   at::Tensor ko;
-  if (k.has_value()) ko = given[1] != nullptr ? *given[1] : at::empty(k->sizes(), k->options());
+  if (k.has_value()) ko = given[1] != nullptr ? *given[1] : empty_on(k->sizes(), at::kBFloat16, k->device());
   if (batch * tokens == 0 || q.size(-2) == 0) return {qo, ko};
   TORCH_CHECK(batch * tokens < (int64_t(1) << 31) && q.size(-2) < (1 << 16) && (!k.has_value() || k->size(-2) < (1 << 16)),
               "too many tokens or heads");
-  TORCH_CHECK(axes >= 1 && axes <= 4, "there must be one to four sections");
   b200attn_qk_norm_rope_args a{};
   a.struct_bytes = sizeof a;
   a.batch = int32_t(batch);
@@ -208,13 +236,7 @@ inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, cons
   a.position_stride_token = pos.stride(-1);
   a.inv_freq = inv_freq.data_ptr<float>();
   a.axes = int32_t(axes);
-  int64_t pairs = 0;
-  for (int64_t i = 0; i < axes; ++i) {
-    TORCH_CHECK(sections[size_t(i)] >= 0 && sections[size_t(i)] <= 64, "sections must be 0 .. 64 pairs");
-    a.section[i] = int32_t(sections[size_t(i)]);
-    pairs += sections[size_t(i)];
-  }
-  TORCH_CHECK(inv_freq.size(0) == pairs, "inv_freq holds ", inv_freq.size(0), " frequencies, sections add up to ", pairs);
+  for (int64_t i = 0; i < axes; ++i) a.section[i] = int32_t(sections[size_t(i)]);
   a.eps = float(eps);
   a.interleaved = interleaved ? 1 : 0;
   a.stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();

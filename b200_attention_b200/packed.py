@@ -132,11 +132,10 @@ class AttentionPlan:
             torch.cuda.current_stream().synchronize()
         i = s.info
         self.rows_q, self.rows_kv = i.rows_q, i.rows_kv
-        self._now = (self.heads, self.heads_kv, i.rows_q, i.rows_kv, self.len_prefix, i.grid, i.units, i.slot_rows)
-
-    def _for_capture(self, k) -> tuple:
-        grid = self._sm_count if self.len_prefix or k.size(0) else 0
-        return (*self._now[:5], grid, self._room_units, self._room_slots)
+        # what calls are told (serving_calls.h): sizes, launch, and the launch of a captured call, for all that a later
+        # table may hold
+        self._now = (self.heads, self.heads_kv, i.rows_q, i.rows_kv, self.len_prefix, i.grid, i.units, i.slot_rows,
+                     self._sm_count, self._room_units, self._room_slots)
 
     def _hold(self, rows_q: int, rows_kv: int) -> None:
         if self._captured is None:
@@ -170,15 +169,9 @@ def _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stre
             raise RuntimeError(f"stream is on {stream.device}, the plan on {plan.device}")
         with torch.cuda.stream(stream):
             return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
-    if torch.cuda.current_device() != plan.device.index:
-        with torch.cuda.device(plan.device):
-            return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
-    # a replay may find the table of other lengths: a captured call launches for all that may be in it
-    capturing = torch.cuda.is_current_stream_capturing()
-    o, lse = (N._direct or N.direct()).attention_planned(
-        q, k, v, k_prefix, v_prefix, plan._table, plan._for_capture(k) if capturing else plan._now, softmax_scale,
-        return_lse, out)
-    if capturing:
+    o, lse, captured = (N._direct or N.direct()).attention_planned(q, k, v, k_prefix, v_prefix, plan._table, plan._now,
+                                                                   softmax_scale, return_lse, out)
+    if captured:
         plan._hold(q.size(0), k.size(0))
     return (o, lse) if return_lse else o
 

@@ -99,10 +99,6 @@ def qk_norm_rope(
         sections = (inv_freq.numel(),)
     elif type(sections) is not tuple:
         sections = tuple(sections)
-    if not 1 <= len(sections) <= 4 or min(sections) < 0 or not 1 <= sum(sections) <= HEAD_DIM // 2:
-        raise ValueError(f"sections must be 1 to 4 counts that add up to 1 .. {HEAD_DIM // 2}, got {sections}")
-    if inv_freq.numel() != sum(sections):
-        raise ValueError(f"inv_freq holds {inv_freq.numel()} frequencies, sections add up to {sum(sections)}")
     q_out = k_out = None
     if out is not None:
         q_out, k_out = out
