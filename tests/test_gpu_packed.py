@@ -174,6 +174,37 @@ def test_strided_operands(ops):
     assert (wide[:, 0] == 7).all() and (wide[:, 9] == 7).all() and (wide[:, :, 128:] == 7).all()
 
 
+def test_result_in_the_place_of_q(ops):
+    """out may be q itself: whole items, cut ones, and rows joined with a prefix."""
+    for lens_q, lens_kv, prefix in [([300, 1, 40], [300, 9, 40], 0), ([1, 2], [9000, 5000], 0), ([1] * 9, [50] * 9, 700)]:
+        q, k, v, kp, vp = make(lens_q, lens_kv, 8, 2, prefix=prefix)
+        plan = ops.AttentionPlan(lens_q, lens_kv, heads=8, heads_kv=2, len_prefix=prefix)
+        call = lambda out: (ops.attention_shared_prefix(q, kp, vp, k, v, plan, out=out) if prefix
+                            else ops.attention_packed(q, k, v, plan, out=out))
+        want = call(torch.empty_like(q))
+        got = call(q)
+        settle()
+        assert got is q or got.data_ptr() == q.data_ptr()
+        assert torch.equal(q, want)
+
+
+def test_a_cache_whose_offsets_pass_32_bits(ops):
+    """Sequences at the end of a cache of 2.3e9 elements (4.6 GB each for k and v)."""
+    heads_kv, rows = 8, 2_250_000
+    lens_q, lens_kv = [1, 20], [700, 333]
+    starts = [rows - 400 - 700, rows - 333]
+    k, v = (torch.empty(rows, heads_kv, 128, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    for t in (k, v):
+        t[:1000] = math.nan
+        t[rows - 2000:] = rand(5 if t is k else 6, 2000, heads_kv, 128)
+    assert starts[0] * heads_kv * 128 > 2**31
+    q = rand(3, sum(lens_q), 16, 128)
+    plan = ops.AttentionPlan(lens_q, lens_kv, heads=16, heads_kv=heads_kv, starts_kv=starts)
+    o, lse = ops.attention_packed(q, k, v, plan, return_lse=True)
+    settle()
+    R.check_attention(o, lse, R.attention(q, k, v, lens_q, lens_kv, causal=True, starts=starts))
+
+
 def test_rows_behind_the_last_sequence_keep_what_they_hold(ops):
     q, k, v, kp, vp = make([3, 2], [9, 2], 4, 2, extra=5, prefix=20)
     out = torch.full_like(q, 3.0)

@@ -141,6 +141,20 @@ def test_strides_streams_and_graphs(ops):
     del graph
 
 
+def test_offsets_past_32_bits(ops):
+    """2.3e9 elements: the last tokens' rows begin behind 2^31."""
+    tokens, heads = 70_001, 256
+    q = torch.empty(tokens, heads, 128, device="cuda", dtype=torch.bfloat16)
+    q[-8:] = rand(1, 8, heads, 128)
+    q[:8] = rand(2, 8, heads, 128)
+    assert (tokens - 8) * heads * 128 > 2**31
+    pos, f = torch.arange(tokens, device="cuda"), freqs((64,))
+    qo, _ = ops.qk_norm_rope(q, None, pos, f)
+    torch.cuda.synchronize()
+    check(qo[-8:], q[-8:], None, pos[None, -8:], f, (64,), False)
+    check(qo[:8], q[:8], None, pos[None, :8], f, (64,), False)
+
+
 def test_values_that_are_not_finite_stay_in_their_head(ops):
     q = rand(1, 5, 4, 128)
     q[2, 1, 7], q[3, 0, 100] = math.nan, math.inf
