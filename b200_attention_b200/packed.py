@@ -209,52 +209,6 @@ def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: t
         raise RuntimeError("this plan has no prefix: use attention_packed")
     if k_prefix is None or v_prefix is None:
         raise TypeError("k_prefix and v_prefix must be torch.Tensors")
-    return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
-    # a replay may find the table of other lengths: a captured call launches for all that may be in it
-    capturing = torch.cuda.is_current_stream_capturing()
-    o, lse = N.torch_ops().attention_planned(q, k, v, k_prefix, v_prefix, plan._table,
-                                             plan._for_capture(k) if capturing else plan._now, softmax_scale,
-                                             return_lse, out)
-    if capturing:
-        plan._hold(q.size(0), k.size(0))
-    return (o, lse) if return_lse else o
-
-
-def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: AttentionPlan, *,
-                     softmax_scale: float = 0.0, return_lse: bool = False, out: Optional[torch.Tensor] = None,
-                     stream: Optional[torch.cuda.Stream] = None):
-    """O = softmax(Q K^T * scale) V for every sequence of the plan, on the current CUDA stream.
-
-    q: [rows, heads, 128] bf16, the sequences' tokens back to back; k, v: [rows, heads_kv, 128]. Any strides that are
-    multiples of 8 elements (at least 128), head_dim dense. Returns O like q and, if asked, LSE [heads, rows] fp32
-    (natural log). A token that sees no key gets O = 0 and LSE = -inf. Rows of q behind the plan's last sequence are
-    not read; their rows of a given `out` keep what they hold, in an O made here they are 0 (LSE: -inf). Rows of
-    k and v outside the plan's sequences have no influence, whatever they hold. `out` must not overlap k or v.
-    Forward only. softmax_scale <= 0: 1 / sqrt(128).
-    """
-    if not isinstance(plan, AttentionPlan):
-        raise TypeError("plan must be an AttentionPlan")
-    if plan.len_prefix:
-        raise RuntimeError("this plan has a prefix: use attention_shared_prefix")
-    return _run(q, k, v, None, None, plan, softmax_scale, return_lse, out, stream)
-
-
-def attention_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor,
-                            v: torch.Tensor, plan: AttentionPlan, *, softmax_scale: float = 0.0,
-                            return_lse: bool = False, out: Optional[torch.Tensor] = None,
-                            stream: Optional[torch.cuda.Stream] = None):
-    """As attention_packed, with every token also seeing all of a prefix [len_prefix, heads_kv, 128] in front of its
-    sequence's own keys. The prefix is read for blocks of tokens of all sequences together, not once per sequence.
-    k_prefix, v_prefix: at least the plan's len_prefix rows (the first ones are used).
-    """
-    if not isinstance(plan, AttentionPlan):
-        raise TypeError("plan must be an AttentionPlan")
-    if not plan.len_prefix:
-        raise RuntimeError("this plan has no prefix: use attention_packed")
-    if k_prefix is None or v_prefix is None:
-        raise TypeError("k_prefix and v_prefix must be torch.Tensors")
-        if t.dim() < 1 or t.size(0) < plan.len_prefix:
-            raise RuntimeError(f"{name} has fewer than the plan's {plan.len_prefix} rows")
     return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream)
 
 

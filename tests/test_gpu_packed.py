@@ -274,6 +274,23 @@ def test_two_streams_and_another_thread_of_work(ops):
         assert all(torch.equal(o, want[i]) for o in got[i])
 
 
+def test_shared_prefix_on_another_stream(ops):
+    lens_q, lens_kv = [1, 2, 1], [50, 130, 9]
+    q, k, v, kp, vp = make(lens_q, lens_kv, 8, 2, prefix=2000)
+    plan = ops.AttentionPlan(lens_q, lens_kv, heads=8, heads_kv=2, len_prefix=2000)
+    want, want_lse = ops.attention_shared_prefix(q, kp, vp, k, v, plan, return_lse=True)
+    settle()
+    s = torch.cuda.Stream()
+    late = torch.empty_like(q)
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)
+        late.copy_(q)  # what the call reads is only written now
+    got, lse = ops.attention_shared_prefix(late, kp, vp, k, v, plan, return_lse=True, stream=s)
+    s.synchronize()
+    assert torch.equal(got, want) and torch.equal(lse, want_lse)
+    settle()
+
+
 def test_captured_call_follows_an_updated_plan(ops):
     q, k, v, kp, vp = make([1] * 4, [600] * 4, 8, 2, prefix=700)
     starts = [0, 600, 1200, 1800]
