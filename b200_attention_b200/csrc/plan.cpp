@@ -22,14 +22,21 @@ constexpr int kTile = 128;
 
 // Costs in thousandths of the time of a K/V tile against two Q tiles (1.6 us), as measured with pieces of equal length.
 // A piece of one Q tile runs on one of a CTA's two lanes: alone it is bound by its chain of steps, beside another lane
-// by what the two share, which is above all memory (64 KB per tile).
+// by what the two share, which is above all memory (64 KB per tile). Next to a prefix, whose pieces load memory on
+// every CTA, a tile costs more of that; without one a CTA that has more tiles than others gets more of the memory's
+// rate, and a piece's start weighs more. One pair of figures for both costs a tenth of the time on one side or the
+// other (10 tokens of 4000 keys, 40 heads: 48.8 us with the first, 41.1 with the second; 90 tokens on a prefix of
+// 3000: 41.0 and 45.4).
 constexpr int64_t kTilePair = 1000;
 constexpr int64_t kTilePairPrefix = 1250;  // the same, with every CTA on keys of its own, which come from memory
 constexpr int64_t kPairStart = 2200;    // Q load, first scores, last PV, stores
-constexpr int64_t kTileShared = 930;
-constexpr int64_t kSharedStart = 750;
+constexpr int64_t kTileSharedPrefix = 930;
+constexpr int64_t kSharedStartPrefix = 750;
+constexpr int64_t kTileShared = 600;
+constexpr int64_t kSharedStart = 1800;
 constexpr int64_t kTileChain = 950;     // scores, softmax, PV of one tile after the other
 constexpr int64_t kChainStart = 1300;
+constexpr int64_t kTilesMemory = 13;    // two tiles of one Q tile, of all CTAs' time together: 128 KB at 6.3 TB/s
 constexpr int64_t kJoin = 2500;         // the second kernel, once,
 constexpr int64_t kJoinRows = 14;       // and per row of partial results, divided by this
 // A piece is walked without a look at the other CTAs, under waits of limited length: keep it below a tenth of a second.
@@ -47,9 +54,10 @@ struct Cost {
   int64_t shared;  // of the CTA's time
   int64_t chain;   // of a lane's time, for one Q tile
 };
-Cost cost_of(const PlanPiece& p, int32_t small_tokens) {
+Cost cost_of(const PlanPiece& p, int32_t small_tokens, bool has_prefix) {
   if (p.tiles[1] > 0) return {2, kPairStart + p.tiles[1] * (p.source == 1 ? kTilePairPrefix : kTilePair), 0};
-  return {p.n_tokens <= small_tokens ? 0 : 1, kSharedStart + p.tiles[0] * kTileShared,
+  return {p.n_tokens <= small_tokens ? 0 : 1,
+          has_prefix ? kSharedStartPrefix + p.tiles[0] * kTileSharedPrefix : kSharedStart + p.tiles[0] * kTileShared,
           kChainStart + p.tiles[0] * kTileChain};
 }
 
@@ -131,7 +139,9 @@ struct Planner {
   bool has_prefix;  // every piece leaves a partial result
   bool by_groups;   // K/V of sixteen heads at a time, where all of it would not stay in L2 (see CausalWalk's groups)
 
-  Cost cost(const Run& r) const { return cost_of(cut_piece(items[size_t(r.item)], r.from, r.len), small_tokens); }
+  Cost cost(const Run& r) const {
+    return cost_of(cut_piece(items[size_t(r.item)], r.from, r.len), small_tokens, has_prefix);
+  }
 
   // Items cut into pieces of at most `len` tiles, not dealt yet.
   Deal uniform(int32_t len) const {
@@ -237,7 +247,7 @@ struct Planner {
       found = std::move(d);
     };
     // Close to what no schedule can beat: not worth the time of looking for another (a decode step plans anew each time).
-    if (!pairs && end <= whole.mean() * 107 / 100) return found;
+    if (!pairs && end <= std::max(whole.mean() * 107 / 100, total_tiles * kTilesMemory / 2)) return found;
     // What a few CTAs have too much. With fewer items than CTAs there is nothing to even out.
     if (pairs && items.size() > size_t(sm_count))
       for (const int64_t percent : {101, 102, 104, 107})
