@@ -49,7 +49,7 @@ constexpr int kPairSlotsP = 2;
 constexpr int kPairBytesP = 2 * kTileBytes;
 constexpr int kPlanThreads = 512;
 // Registers per thread of the three kinds of warps (128 in the mean). Against 184 / 64 / 80: 3 % at 8 prompts of 1 to
-// 8192 tokens; against 192 / 56 / 72: 2 %, the MMA warp then spills.
+// 8192 tokens; against 192 / 56 / 72: 2 %.
 constexpr int kPlanRegsSoftmax = 192;
 constexpr int kPlanRegsEpilogue = 48;
 constexpr int kPlanRegsOther = 80;

@@ -5,6 +5,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -41,8 +42,9 @@ inline void check_rows(const char* name, const at::Tensor& t, int64_t heads, con
 inline b200attn_operand row_operand(const at::Tensor& t) { return {t.data_ptr(), 0, t.stride(1), t.stride(0)}; }
 
 // What a plan says to a call: heads, heads_kv, rows_q, rows_kv, len_prefix, grid, join units, slot rows; then grid, join
-// units and slot rows for a call that is being captured, whose replays may find the table of other lengths.
-constexpr size_t kPlanInts = 11;
+// units and slot rows for a call that is being captured, whose replays may find the table of other lengths; last, the
+// stream that the table was allocated on.
+constexpr size_t kPlanInts = 12;
 
 inline at::Tensor empty_on(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
   return at::detail::empty_cuda(sizes, type, device, std::nullopt);
@@ -52,6 +54,11 @@ inline bool capturing(cudaStream_t stream) {
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
   C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &status));
   return status != cudaStreamCaptureStatusNone;
+}
+
+// A tensor that the caller gave as output: a backward pass that saved it must see that it has changed.
+inline void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // Returns O, LSE (or an undefined tensor), and whether the call was captured.
@@ -129,6 +136,12 @@ inline std::tuple<at::Tensor, at::Tensor, bool> attention_planned(const at::Tens
   a.slot_rows = slots;
   a.stream = stream;
   check_rc(b200attn_forward_planned(&a));
+  if (out.has_value()) written(o);
+  // A plan may go, or take another table, while a call on another stream than the table's own still reads it. (The table
+  // of a captured call stays.)
+  if (!captured && reinterpret_cast<int64_t>(stream) != plan[11])
+    c10::cuda::CUDACachingAllocator::recordStream(table.storage().data_ptr(),
+                                                  c10::cuda::getCurrentCUDAStream(device.index()));
   return {o, lse, captured};
 }
 
@@ -169,6 +182,7 @@ inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, cons
   check_tokens("q", q, nullptr);
   if (k.has_value()) check_tokens("k", *k, &q);
   TORCH_CHECK(k.has_value() || !k_weight.has_value(), "k_weight is given without k");
+  TORCH_CHECK(q.size(-2) > 0 || !k.has_value() || k->size(-2) == 0, "q has no heads, k has ", k.has_value() ? k->size(-2) : 0);
   const int64_t batch = q.dim() == 4 ? q.size(0) : 1, tokens = q.size(-3);
   TORCH_CHECK(positions.device() == q.device() && inv_freq.device() == q.device(),
               "positions and inv_freq must be on q's device");
@@ -241,6 +255,8 @@ inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, cons
   a.interleaved = interleaved ? 1 : 0;
   a.stream = c10::cuda::getCurrentCUDAStream(q.device().index()).stream();
   check_rc(b200attn_qk_norm_rope(&a));
+  if (given[0] != nullptr) written(qo);
+  if (given[1] != nullptr && a.heads_k > 0) written(ko);
   return {qo, ko};
 }
 

@@ -17,6 +17,7 @@ The reference project has no counterpart: its kernels take one rectangular probl
 from __future__ import annotations
 
 import ctypes as C
+import operator
 from typing import Optional
 
 import torch
@@ -54,11 +55,13 @@ class Schedule:
         for name, vals, top in (("lens_q", lq, 2**30), ("lens_kv", lk, 2**30), ("starts_kv", st or (), 2**31)):
             if any(not 0 <= x < top for x in vals):
                 raise ValueError(f"{name} must be 0 .. {top - 1}")
+        heads, len_prefix = operator.index(heads), operator.index(len_prefix)
+        heads_kv = heads if heads_kv is None else operator.index(heads_kv)
         for name, x in (("heads", heads), ("heads_kv", heads_kv), ("len_prefix", len_prefix)):
-            if x is not None and not -2**31 <= x < 2**31:
+            if not -2**31 <= x < 2**31:
                 raise ValueError(f"{name} is out of range")
-        self.sequences, self.heads, self.heads_kv = len(lq), int(heads), int(heads if heads_kv is None else heads_kv)
-        self.causal, self.len_prefix = bool(causal), int(len_prefix)
+        self.sequences, self.heads, self.heads_kv = len(lq), heads, heads_kv
+        self.causal, self.len_prefix = bool(causal), len_prefix
         n = max(1, len(lq))
         d = N.PlanDesc()
         d.struct_bytes = C.sizeof(N.PlanDesc)
@@ -121,8 +124,12 @@ class AttentionPlan:
         self._room_units = 2 * s.info.units + 1024
         self._room_slots = 2 * s.info.slot_rows + 4096
         self._captured = None  # (rows of q, rows of k) that every captured call has at least
-        self._table = torch.zeros(2 * s.table.numel() + 16384, dtype=torch.int32, device=device)
+        self._new_table(s)
         self._put(s)
+
+    def _new_table(self, s: Schedule) -> None:
+        self._table = torch.zeros(2 * s.table.numel() + 16384, dtype=torch.int32, device=self.device)
+        self._table_stream = torch.cuda.current_stream(self.device).cuda_stream
 
     def _put(self, s: Schedule) -> None:
         with torch.cuda.device(self.device):
@@ -132,10 +139,10 @@ class AttentionPlan:
             torch.cuda.current_stream().synchronize()
         i = s.info
         self.rows_q, self.rows_kv = i.rows_q, i.rows_kv
-        # what calls are told (serving_calls.h): sizes, launch, and the launch of a captured call, for all that a later
-        # table may hold
+        # what calls are told (serving_calls.h): sizes, launch, the launch of a captured call, for all that a later
+        # table may hold, and where the table was allocated
         self._now = (self.heads, self.heads_kv, i.rows_q, i.rows_kv, self.len_prefix, i.grid, i.units, i.slot_rows,
-                     self._sm_count, self._room_units, self._room_slots)
+                     self._sm_count, self._room_units, self._room_slots, self._table_stream)
 
     def _hold(self, rows_q: int, rows_kv: int) -> None:
         if self._captured is None:
@@ -159,7 +166,7 @@ class AttentionPlan:
                                    "capture again")
         elif not fits:
             self._room_units, self._room_slots = 2 * s.info.units + 1024, 2 * s.info.slot_rows + 4096
-            self._table = torch.zeros(2 * s.table.numel() + 16384, dtype=torch.int32, device=self.device)
+            self._new_table(s)
         self._put(s)
 
 

@@ -291,6 +291,40 @@ def test_shared_prefix_on_another_stream(ops):
     settle()
 
 
+def test_a_plan_may_go_while_another_stream_uses_it(ops):
+    lens_q, lens_kv = [1, 2, 1], [50, 130, 9]
+    q, k, v, _, _ = make(lens_q, lens_kv, 8, 2)
+    plan = ops.AttentionPlan(lens_q, lens_kv, heads=8, heads_kv=2)
+    want = ops.attention_packed(q, k, v, plan)
+    settle()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(40_000_000)
+    got = ops.attention_packed(q, k, v, plan, stream=s)
+    place, size = plan._table.data_ptr(), plan._table.numel()
+    del plan
+    others = [torch.zeros(size, dtype=torch.int32, device="cuda") for _ in range(4)]
+    assert not s.query(), "the call was to be waiting still"
+    assert place not in [t.data_ptr() for t in others]
+    s.synchronize()
+    assert torch.equal(got, want)
+    settle()
+
+
+def test_given_outputs_count_as_changed(ops):
+    q, k, v, _, _ = make([3], [5], 4, 2)
+    plan = ops.AttentionPlan([3], [5], heads=4, heads_kv=2)
+    w = torch.ones(4, 128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    saved = (q * w).sum()  # keeps q for the gradient of w
+    ops.attention_packed(q, k, v, plan, out=q)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    with torch.inference_mode():
+        o = torch.empty_like(q)
+        ops.attention_packed(q, k, v, plan, out=o)
+    settle()
+
+
 def test_captured_call_follows_an_updated_plan(ops):
     q, k, v, kp, vp = make([1] * 4, [600] * 4, 8, 2, prefix=700)
     starts = [0, 600, 1200, 1800]

@@ -172,6 +172,24 @@ def test_empty(ops):
     assert qo.shape == q.shape and ko.shape == (0, 2, 128)
 
 
+def test_keys_need_queries(ops):
+    pos, f = torch.arange(6, device="cuda"), freqs((64,))
+    with pytest.raises(RuntimeError, match="q has no heads"):
+        ops.qk_norm_rope(rand(1, 6, 0, 128), rand(2, 6, 2, 128), pos, f)
+    qo, ko = ops.qk_norm_rope(rand(1, 6, 4, 128), rand(2, 6, 0, 128), pos, f)
+    assert qo.shape == (6, 4, 128) and ko.shape == (6, 0, 128)
+
+
+def test_given_outputs_count_as_changed(ops):
+    q, k, pos, f = rand(1, 6, 4, 128), rand(2, 6, 2, 128), torch.arange(6, device="cuda"), freqs((64,))
+    w = torch.ones(128, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    saved = [(q * w).sum(), (k * w).sum()]  # keep q and k for the gradient of w
+    ops.qk_norm_rope(q, k, pos, f, out=(q, k))
+    for y in saved:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+
+
 def test_refusals(ops):
     q, k, pos, f = rand(1, 6, 4, 128), rand(2, 6, 2, 128), torch.arange(6, device="cuda"), freqs((64,))
     w = rand(3, 128)

@@ -172,6 +172,12 @@ def test_plans_refused(native_built, kw, error):
         packed.Schedule(lens_q, lens_kv, **args)
 
 
+@pytest.mark.parametrize("kw", [dict(heads=2.5), dict(heads=4, heads_kv=2.0), dict(heads=4, len_prefix=1.5), dict(heads="4")])
+def test_plans_take_integers_only(native_built, kw):
+    with pytest.raises(TypeError):
+        packed.Schedule([4], [4], **kw)
+
+
 def test_plan_needs_a_cuda_device(native_built):
     with pytest.raises(RuntimeError, match="no CPU path"):
         ops.AttentionPlan([1], [1], heads=1, device="cpu")
