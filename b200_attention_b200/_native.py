@@ -121,6 +121,8 @@ class PlanInfo(C.Structure):
         ("grid", C.c_int32),
         ("pieces", C.c_int32),
         ("units", C.c_int32),
+        ("wide_pieces", C.c_int32),
+        ("reserved", C.c_int32),
         ("rows_q", C.c_int64),
         ("rows_kv", C.c_int64),
         ("slot_rows", C.c_int64),
@@ -150,7 +152,7 @@ class PlannedArgs(C.Structure):
         ("lse", C.c_void_p),
         ("lse_stride_head", C.c_int64),
         ("softmax_scale", C.c_float),
-        ("reserved2", C.c_int32),
+        ("wide_pieces", C.c_int32),
         ("table", C.c_void_p),
         ("workspace", C.c_void_p),
         ("slot_rows", C.c_int64),

@@ -74,6 +74,8 @@ int b200attn_plan_create(const b200attn_plan_desc* d, b200attn_plan_info* info, 
     info->grid = plan->grid;
     info->pieces = plan->pieces;
     info->units = plan->units;
+    info->wide_pieces = plan->wide_pieces;
+    info->reserved = 0;
     info->rows_q = plan->rows_q;
     info->rows_kv = plan->rows_kv;
     info->slot_rows = plan->slot_rows;
@@ -106,7 +108,7 @@ int b200attn_forward_planned(const b200attn_planned_args* a) {
   if (a == nullptr) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "args is null");
   if (a->struct_bytes != sizeof *a)
     return fail(B200ATTN_ERR_INVALID_ARGUMENT, "struct_bytes does not match this library's b200attn_planned_args");
-  if (a->reserved != 0 || a->reserved2 != 0) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "reserved fields must be 0");
+  if (a->reserved != 0) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "reserved fields must be 0");
   if (a->head_dim != kHeadDim) return fail(B200ATTN_ERR_UNSUPPORTED, "head_dim must be 128");
   if (a->heads < 1 || a->heads_kv < 1 || a->heads % a->heads_kv != 0)
     return fail(B200ATTN_ERR_INVALID_ARGUMENT, "heads must be a positive multiple of heads_kv");
@@ -183,7 +185,7 @@ int b200attn_forward_planned(const b200attn_planned_args* a) {
     // a pair that has no rows is not read; its maps are the other pair's
     if (a->rows_kv == 0) maps.k = maps.k_prefix, maps.v = maps.v_prefix;
     if (a->len_prefix == 0) maps.k_prefix = maps.k, maps.v_prefix = maps.v;
-    const cudaError_t e = launch_plan(maps, p, a->grid, stream);
+    const cudaError_t e = launch_plan(maps, p, a->grid, a->wide_pieces > 0, stream);
     if (e != cudaSuccess) return fail_cuda("kernel launch", e);
     g_launches.fetch_add(1, std::memory_order_relaxed);
   }

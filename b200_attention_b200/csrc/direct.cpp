@@ -40,9 +40,9 @@ bool truth(PyObject* o) {
   return v != 0;
 }
 
-c10::SmallVector<int64_t, 12> integers(PyObject* o, const char* name) {
+c10::SmallVector<int64_t, 16> integers(PyObject* o, const char* name) {
   TORCH_CHECK_TYPE(PyTuple_Check(o), name, " must be a tuple");
-  c10::SmallVector<int64_t, 12> out;
+  c10::SmallVector<int64_t, 16> out;
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(o); ++i) out.push_back(integer(PyTuple_GET_ITEM(o, i)));
   return out;
 }

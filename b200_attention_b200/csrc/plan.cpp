@@ -370,6 +370,7 @@ std::string plan_build(const PlanInput& in, Plan* plan) {
       const Run& r = deal.runs[size_t(by_item[k])];
       PlanPiece& p = pieces[size_t(by_item[k])];
       p = cut_piece(items[i], r.from, r.len);
+      plan->wide_pieces += p.tiles[1] > 0 ? 1 : 0;
       if (!partial) continue;
       p.slot_row = int32_t(slots);
       slots += int64_t(items[i].n_tokens) * group;

@@ -65,6 +65,7 @@ struct Plan {
   int32_t grid = 0;       // CTAs that have a piece
   int32_t pieces = 0;
   int32_t units = 0;
+  int32_t wide_pieces = 0;  // of two Q tiles
   int64_t slot_rows = 0;  // rows of fp32 partials that the pieces write
   int64_t rows_q = 0;     // rows of q and o that the plan covers
   int64_t rows_kv = 0;    // rows of k and v that it may read: past the last key of any sequence

@@ -30,7 +30,7 @@ struct PlanParams {
 };
 
 cudaError_t prepare_plan_kernels();
-cudaError_t launch_plan(const PlanMaps& maps, const PlanParams& p, int grid, cudaStream_t stream);
+cudaError_t launch_plan(const PlanMaps& maps, const PlanParams& p, int grid, bool wide, cudaStream_t stream);
 cudaError_t launch_plan_join(const PlanParams& p, int grid, cudaStream_t stream);
 
 }  // namespace b200attn

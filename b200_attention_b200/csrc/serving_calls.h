@@ -43,8 +43,8 @@ inline b200attn_operand row_operand(const at::Tensor& t) { return {t.data_ptr(),
 
 // What a plan says to a call: heads, heads_kv, rows_q, rows_kv, len_prefix, grid, join units, slot rows; then grid, join
 // units and slot rows for a call that is being captured, whose replays may find the table of other lengths; last, the
-// stream that the table was allocated on.
-constexpr size_t kPlanInts = 12;
+// stream that the table was allocated on, and the plan's wide pieces.
+constexpr size_t kPlanInts = 13;
 
 inline at::Tensor empty_on(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) {
   return at::detail::empty_cuda(sizes, type, device, std::nullopt);
@@ -118,6 +118,7 @@ inline std::tuple<at::Tensor, at::Tensor, bool> attention_planned(const at::Tens
   a.len_prefix = int32_t(len_prefix);
   a.grid = int32_t(grid);
   a.join_units = int32_t(units);
+  a.wide_pieces = int32_t(plan[12]);
   a.q = row_operand(q);
   a.k = row_operand(k);
   a.v = row_operand(v);

@@ -140,9 +140,10 @@ class AttentionPlan:
         i = s.info
         self.rows_q, self.rows_kv = i.rows_q, i.rows_kv
         # what calls are told (serving_calls.h): sizes, launch, the launch of a captured call, for all that a later
-        # table may hold, and where the table was allocated
+        # table may hold, where the table was allocated, and which build of the kernel is the faster one
         self._now = (self.heads, self.heads_kv, i.rows_q, i.rows_kv, self.len_prefix, i.grid, i.units, i.slot_rows,
-                     self._sm_count, self._room_units, self._room_slots, self._table_stream)
+                     self._sm_count, self._room_units, self._room_slots, self._table_stream,
+                     i.wide_pieces)
 
     def _hold(self, rows_q: int, rows_kv: int) -> None:
         if self._captured is None:

@@ -214,6 +214,8 @@ typedef struct b200attn_plan_info {
   int32_t grid;          /* CTAs with work */
   int32_t pieces;        /* pieces of work */
   int32_t units;         /* groups of rows that are joined from partial results */
+  int32_t wide_pieces;   /* pieces of more than 128 rows (tokens x heads of a group), as prompts have */
+  int32_t reserved;
   int64_t rows_q;        /* rows of q and o that the plan covers */
   int64_t rows_kv;       /* rows of k and v that it may read */
   int64_t slot_rows;     /* rows of partial results */
@@ -241,7 +243,7 @@ typedef struct b200attn_planned_args {
   float* lse;              /* [heads, >= rows_q] fp32, natural log; may be NULL */
   int64_t lse_stride_head; /* elements between heads of lse */
   float softmax_scale;     /* <= 0 selects 1/sqrt(head_dim) */
-  int32_t reserved2;       /* 0 */
+  int32_t wide_pieces;     /* info.wide_pieces: chooses the faster of two builds of the kernel; either is right */
   const void* table;       /* device memory, 16-byte aligned */
   void* workspace;         /* device memory, 32-byte aligned, slot_rows * 516 bytes, any contents; calls
                             * that may overlap need workspaces of their own */

@@ -245,6 +245,26 @@ def test_more_pieces_than_a_cta_keeps_at_hand(ops):
     run_case(ops, lens, lens, 4, 4)
 
 
+@pytest.mark.parametrize("lens_q, lens_kv, prefix", [([1, 40, 300, 5], [700, 40, 900, 131], 0), ([1] * 40, [300] * 40, 0), ([70, 1], [70, 130], 600)])
+def test_both_builds_of_the_kernel_take_every_plan(ops, lens_q, lens_kv, prefix):
+    """Whichever the plan asks for (by its wide pieces): a captured call keeps the one that it was captured with."""
+    q, k, v, kp, vp = make(lens_q, lens_kv, 8, 2, prefix=prefix)
+    plan = ops.AttentionPlan(lens_q, lens_kv, heads=8, heads_kv=2, len_prefix=prefix)
+    wide = plan._now[-1]
+    assert (wide > 0) == (max(lens_q) > 32 or prefix > 0)  # 32 tokens x 4 heads of a group fill a Q tile
+    results = []
+    for hint in (wide, 0, 1):
+        plan._now = (*plan._now[:-1], hint)
+        if prefix:
+            results.append(ops.attention_shared_prefix(q, kp, vp, k, v, plan, return_lse=True))
+        else:
+            results.append(ops.attention_packed(q, k, v, plan, return_lse=True))
+        settle()
+    R.check_attention(*results[0], R.attention(q, k, v, lens_q, lens_kv, causal=True, k_prefix=kp, v_prefix=vp))
+    for o, lse in results[1:]:
+        assert torch.equal(o, results[0][0]) and torch.equal(lse, results[0][1])
+
+
 def test_agrees_with_the_rectangular_call(ops):
     b, n = 3, 640
     q, k, v = rand(1, b * n, 8, 128), rand(2, b * n, 2, 128), rand(3, b * n, 2, 128)

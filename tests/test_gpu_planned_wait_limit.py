@@ -25,6 +25,7 @@ def args_for(N, q, k, v, o, schedule, table):
     a.heads, a.heads_kv, a.head_dim = q.shape[1], k.shape[1], 128
     a.rows_q, a.rows_kv = q.shape[0], k.shape[0]
     a.grid, a.join_units, a.slot_rows = schedule.info.grid, schedule.info.units, schedule.info.slot_rows
+    a.wide_pieces = schedule.info.wide_pieces
     for name, t in (("q", q), ("k", k), ("v", v), ("o", o)):
         setattr(a, name, N.Operand(t.data_ptr(), 0, t.stride(1), t.stride(0)))
     a.table = table.data_ptr()
