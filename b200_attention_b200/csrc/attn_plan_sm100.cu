@@ -31,7 +31,7 @@
 //       1.46 M cycles, tensor pipe busy 63 % of them: bound by the chain, as attn_fwd_ws_kernel (1.45 M) is
 //   64 single tokens, 32 + 8 heads, 100-12000 keys  0.23 ms, 6.1 TB/s: bound by memory
 //   64 tokens behind 32768 shared rows, 32 + 8 heads, up to 1024 keys of their own    70 us, 3.8 TB/s: half the CTAs
-//       work on the prefix (chain), half on short runs of keys that each start anew (latency of memory)
+//       work on the prefix (chain), half on short runs of keys that each start anew (see NotedWait)
 //   one token, 128 keys                             5 us: load, scores, softmax, product, store one after the other
 // Asked for and not kept, being slower: K/V tiles prefetched into the L2 two to six ahead (single tokens 235 -> 289 us and
 // more), a third slot in the K/V ring for CTAs of small pieces (228 -> 232 us), boxes of 32 rows for the tile in which a
