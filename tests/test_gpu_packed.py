@@ -214,6 +214,17 @@ def test_rows_behind_the_last_sequence_keep_what_they_hold(ops):
     assert (out[5:] == 3).all() and torch.isfinite(out[:5]).all()
 
 
+def test_a_row_that_sees_one_key_is_its_value(ops):
+    """One probability of exactly 1: nothing is rounded on the way, whatever the score."""
+    lens = [1, 7, 1, 300, 64]
+    q, k, v, _, _ = make(lens, lens, 8, 2)
+    plan = ops.AttentionPlan(lens, lens, heads=8, heads_kv=2)
+    o = ops.attention_packed(q * 3, k, v, plan)
+    settle()
+    first = R.starts_of(lens)
+    assert torch.equal(o[first], v[first].repeat_interleave(4, dim=1))
+
+
 def test_results_repeat(ops):
     lens_q, lens_kv = [1] * 9 + [64], [1 + 700 * i for i in range(9)] + [64]
     q, k, v, kp, vp = make(lens_q, lens_kv, 16, 4, prefix=3500)
