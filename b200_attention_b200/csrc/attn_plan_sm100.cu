@@ -626,15 +626,15 @@ __device__ __forceinline__ void store_result(const PlanParams& p, const PlanPiec
 }
 
 // ---- softmax: one row per thread -------------------------------------------------------------------------
-// As in attn_fwd_ws_kernel: speculative against the row's reference maximum, exact where the tile's sum says that it
-// has to move. Two differences. The first tile speculates too, on a reference of 0: any reference within 2^32 of the
-// true one serves, so the tile stands if its sum lies between 2^-32 and 2^32, and the pass over it for its maximum is
-// only needed for larger scores (it costs a third of a tile's time, which a piece of a few tiles feels). A first tile
-// of which rows see a part only is taken with its maximum all the same: the largest probability of a row is then 1 and
-// loses nothing when it is rounded to bf16, which with few keys is much of the result's error (1 to 40 keys: 0.0023 ->
-// 0.0018 of the result's norm, of which rounding the result itself is 0.0016; from 200 keys on 0.0023 either way). And rows that
-// see no key of a tile, or of the whole piece: their m becomes -inf, which sends them down the exact path, where it is
-// subtracted as 0 so that every probability is 2^-inf = 0.
+// As in attn_fwd_ws_kernel: the first tile is taken with its maximum, later ones speculate against the row's reference
+// and go the exact way where the tile's sum says that it has to move. The maximum comes first because the largest
+// probability of a row is then 2^0 = 1 and loses nothing when it is rounded to bf16: where one key of the first tile
+// outweighs the others (its score 9 to 15, theirs about N(0, 1)) a reference of 0 rounds all of the row's result once
+// more, by up to 2^-8 (error against 64 bits 0.0021 -> 0.0013 of the norm at 128 keys, 0.0024 -> 0.0017 at 1024), and
+// with a few keys so it does for any scores. It costs a part of one tile's time per piece: 148 tokens of 128 keys 26.2
+// -> 27.3 us, of 256 34.5 -> 35.3, of 300 46.2 -> 46.9, 64 of 100-2000 53.1 -> 53.4, whole prompts within 1 %.
+// One difference: rows that see no key of a tile, or of the whole piece. Their m becomes -inf, which sends them down the
+// exact path, where it is subtracted as 0 so that every probability is 2^-inf = 0.
 template <class Wait>
 __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t bar0, uint32_t tmem_base, int q,
                                   int warp_in_group, int lane, Wait& w) {
@@ -689,10 +689,10 @@ __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t ba
         tmem_ld32(s_tmem + 96, s[3]);
         const bool tail = i * kBlockN + kBlockN - 1 > tile_limit;  // uniform across the warp
         const int valid = row_limit - i * kBlockN + 1;             // keys of this tile that the row sees
-        if (tail) {
+        if (tail || i == 0) {
           tmem_wait_ld();
-          mask_tail(s, valid);
-          if (i == 0) m = row_max(s) * scale_log2;  // few keys: see above
+          if (tail) mask_tail(s, valid);
+          if (i == 0) m = row_max(s) * scale_log2;
         }
 
         uint32_t packed[4][16];
@@ -707,7 +707,7 @@ __device__ void plan_softmax_role(const PlanParams& p, PlanAux* aux, uint32_t ba
         }
         float tile_sum = f2_hsum(sum_a, sum_b);
         // written so that a NaN sum also lands on the exact path
-        const bool stands = tile_sum < sum_limit && (i > 0 || tile_sum > 1.0f / sum_limit);
+        const bool stands = tile_sum < sum_limit;
         if (__builtin_expect(__any_sync(0xffffffffu, row_live && !stands), 0)) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) tmem_ld32(s_tmem + c * 32, s[c]);
