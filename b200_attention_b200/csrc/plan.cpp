@@ -220,10 +220,11 @@ struct Planner {
       pairs = pairs || it.tiles1 > 0;
     }
     for (const Item& it : items) long_items += 2 * it.longest() > longest ? 1 : 0;
+    const int32_t uncut = std::min(longest, kLongestPiece);  // what is left whole where it can be
     std::vector<int32_t> lens;
     auto consider = [&](int64_t len) {
       len = std::max<int64_t>(1, len);
-      if (len < longest && std::find(lens.begin(), lens.end(), int32_t(len)) == lens.end()) lens.push_back(int32_t(len));
+      if (len < uncut && std::find(lens.begin(), lens.end(), int32_t(len)) == lens.end()) lens.push_back(int32_t(len));
     };
     const int64_t even = (total_tiles + sm_count - 1) / sm_count;
     for (const int64_t parts : {1, 2, 4, 8}) consider((even + parts - 1) / parts);
@@ -235,8 +236,7 @@ struct Planner {
       if (n > 1) consider((longest + n - 1) / n);
     }
 
-    longest = std::min(longest, kLongestPiece);
-    Deal found = uniform(longest);
+    Deal found = uniform(uncut);
     deal(&found);
     int64_t end = found.end() + join(found);
     const Deal whole = found;
