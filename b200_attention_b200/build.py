@@ -98,7 +98,7 @@ def _build_torch_lib(src: Path, out: Path, force: bool, verbose: bool, python: b
     if python:
         cflags = [*cflags, f"-I{sysconfig.get_paths()['include']}", "-fvisibility=hidden"]
         ldflags = [*ldflags, "-ltorch_python", "-ltorch_cuda", "-L/usr/local/cuda/lib64", "-lcudart"]
-    digest = _digest([src, CSRC / "serving_calls.h", INCLUDE / "b200_attention.h"], tver + " ".join(cflags))
+    digest = _digest([src, CSRC / "serving_calls.h", CSRC / "overlap.h", INCLUDE / "b200_attention.h"], tver + " ".join(cflags))
     if force or _stale(out, digest):
         _run([os.environ.get("CXX", "g++"), *cflags, "-o", out, src, *ldflags], verbose)
         out.with_suffix(".so.sha256").write_text(digest)

@@ -86,7 +86,26 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The rules on where an output may lie, for tensors of any device.
+PyObject* may_overlap(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 2, "may_overlap takes 2 arguments");
+  return PyBool_FromLong(b200attn_torch::may_overlap(tensor(a[0], "a"), tensor(a[1], "b")) ? 1 : 0);
+  END_HANDLE_TH_ERRORS
+}
+
+// out, the input that it may be, another input
+PyObject* check_place(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 3, "check_place takes 3 arguments");
+  b200attn_torch::check_place("out", tensor(a[0], "out"), "q", &tensor(a[1], "q"), {{"k", &tensor(a[2], "k")}});
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"may_overlap", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&may_overlap)), METH_FASTCALL, nullptr},
+    {"check_place", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&check_place)), METH_FASTCALL, nullptr},
     {"attention_planned", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&attention_planned)), METH_FASTCALL, nullptr},
     {"qk_norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&qk_norm_rope)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -15,6 +15,7 @@
 #include <tuple>
 
 #include "../../include/b200_attention.h"
+#include "overlap.h"
 
 namespace b200attn_torch {
 
@@ -88,6 +89,9 @@ inline std::tuple<at::Tensor, at::Tensor, bool> attention_planned(const at::Tens
                     out->stride(2) == 1,
                 "out must match q in shape, dtype and device with a dense head_dim axis");
     check_bf16("out", *out);
+    // A CTA stores rows while others still load theirs.
+    check_place("out", *out, "q", &q, {{"k", &k}, {"v", &v}, {"k_prefix", len_prefix > 0 ? &*k_prefix : nullptr},
+                                       {"v_prefix", len_prefix > 0 ? &*v_prefix : nullptr}});
   }
 
   c10::cuda::CUDAGuard guard(device);

@@ -193,7 +193,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
     multiples of 8 elements (at least 128), head_dim dense. Returns O like q and, if asked, LSE [heads, rows] fp32
     (natural log). A token that sees no key gets O = 0 and LSE = -inf. Rows of q behind the plan's last sequence are
     not read; their rows of a given `out` keep what they hold, in an O made here they are 0 (LSE: -inf). Rows of
-    k and v outside the plan's sequences have no influence, whatever they hold. `out` must not overlap k or v.
+    k and v outside the plan's sequences have no influence, whatever they hold. `out` may be q itself, and otherwise
+    must not overlap q, k, v or a prefix, nor itself.
     Forward only. softmax_scale <= 0: 1 / sqrt(128).
     """
     if not isinstance(plan, AttentionPlan):

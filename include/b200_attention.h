@@ -239,7 +239,8 @@ typedef struct b200attn_planned_args {
   int32_t join_units; /* info.units, or more in the same way; 0: nothing is joined */
   int32_t reserved;   /* 0 */
   b200attn_operand q, k, v, k_prefix, v_prefix; /* bf16; stride_batch is not used */
-  b200attn_operand o;                           /* bf16, written */
+  b200attn_operand o;                           /* bf16, written; may be q itself (pointer and strides), must
+                                                 * otherwise overlap none of the inputs, nor itself (not checked) */
   float* lse;              /* [heads, >= rows_q] fp32, natural log; may be NULL */
   int64_t lse_stride_head; /* elements between heads of lse */
   float softmax_scale;     /* <= 0 selects 1/sqrt(head_dim) */

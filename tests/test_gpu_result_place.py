@@ -1,0 +1,58 @@
+"""GPU tests: where the result of a packed or shared-prefix call may lie, and that other places are refused."""
+
+import pytest
+import torch
+
+from tests import packed_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def rand(seed, *shape):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda", dtype=torch.bfloat16)
+
+
+def test_results_that_overlap_what_is_read_are_refused(native_built):
+    from b200_attention_b200 import _native, ops
+
+    rows = rand(1, 60, 4 + 2 + 2, 128)
+    before = rows.clone()
+    q, k, v = rows[:, :4], rows[:, 4:6], rows[:, 6:]
+    plan = ops.AttentionPlan([40, 20], [40, 20], heads=4, heads_kv=2)
+    behind = ops.AttentionPlan([40, 20], [40, 20], heads=4, heads_kv=2, len_prefix=30)
+    prefix = rand(2, 120, 2, 128)
+    twice = torch.zeros(61 * 512, device="cuda", dtype=torch.bfloat16)
+    bad = [
+        lambda: ops.attention_packed(q[:59], k, v, ops.AttentionPlan([59], [59], heads=4, heads_kv=2), out=rows[1:, :4]),
+        lambda: ops.attention_packed(q, k, v, plan, out=rows[:, 1:5]),
+        lambda: ops.attention_packed(q, k, v, plan, out=rows[:, 4:]),
+        lambda: ops.attention_packed(q.contiguous(), k, v, plan, out=q.contiguous()[:, :1].expand(60, 4, 128)),
+        lambda: ops.attention_packed(q.contiguous(), k, v, plan, out=twice.as_strided((60, 4, 128), (256, 128, 1))),
+        lambda: ops.attention_shared_prefix(q, prefix[:60], prefix[60:], k, v, behind, out=prefix.view(60, 4, 128)),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError, match="overlaps|share memory"):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    torch.cuda.synchronize()
+    assert torch.equal(rows, before)
+    _native.device_check()
+
+
+def test_results_beside_the_inputs_or_in_the_place_of_q(native_built):
+    """Columns of the same rows that nothing is read from, and q itself."""
+    from b200_attention_b200 import _native, ops
+
+    lens = [40, 1, 20]
+    rows = rand(3, 61, 4 + 2 + 2 + 4, 128)
+    q, k, v, beside = rows[:, :4], rows[:, 4:6], rows[:, 6:8], rows[:, 8:]
+    plan = ops.AttentionPlan(lens, lens, heads=4, heads_kv=2)
+    ref = R.attention(q, k, v, lens, lens, causal=True)
+    for out in (beside, q):
+        got = ops.attention_packed(q, k, v, plan, out=out)
+        torch.cuda.synchronize()
+        assert got is out or got.data_ptr() == out.data_ptr()
+        R.check_attention(got, None, ref)
+    _native.device_check()
