@@ -94,6 +94,20 @@ PyObject* may_overlap(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* same_place(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 2, "same_place takes 2 arguments");
+  return PyBool_FromLong(b200attn_torch::same_place(tensor(a[0], "a"), tensor(a[1], "b")) ? 1 : 0);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* dense_apart(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 1, "dense_apart takes 1 argument");
+  return PyBool_FromLong(b200attn_torch::dense_apart(tensor(a[0], "t")) ? 1 : 0);
+  END_HANDLE_TH_ERRORS
+}
+
 // out, the input that it may be, another input
 PyObject* check_place(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -105,6 +119,8 @@ PyObject* check_place(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"may_overlap", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&may_overlap)), METH_FASTCALL, nullptr},
+    {"same_place", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&same_place)), METH_FASTCALL, nullptr},
+    {"dense_apart", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dense_apart)), METH_FASTCALL, nullptr},
     {"check_place", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&check_place)), METH_FASTCALL, nullptr},
     {"attention_planned", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&attention_planned)), METH_FASTCALL, nullptr},
     {"qk_norm_rope", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&qk_norm_rope)), METH_FASTCALL, nullptr},

@@ -9,43 +9,17 @@ import torch
 
 from . import _native as N
 
-HEAD_DIM = 128
-
-
 def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return a.data_ptr() == b.data_ptr() and all(n == 1 or s == u for n, s, u in zip(a.shape, a.stride(), b.stride()))
-
-
-def _span(t: torch.Tensor) -> Tuple[int, int]:
-    first = t.data_ptr()
-    return first, first + 2 * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+    return N.direct().same_place(a, b)
 
 
 def _may_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """False where two tensors cannot share an element: apart as a whole, or heads side by side in the same rows."""
-    (a0, a1), (b0, b1) = _span(a), _span(b)
-    if a1 <= b0 or b1 <= a0:
-        return False
-    if a.shape[:-2] == b.shape[:-2] and a.stride()[:-2] == b.stride()[:-2] and a.stride()[-2] == b.stride()[-2]:
-        # the same rows, every row denser than the step to the next one: columns decide
-        rows = [s for n, s in zip(a.shape[:-2], a.stride()[:-2]) if n > 1]
-        width_a = 2 * ((a.size(-2) - 1) * a.stride(-2) + HEAD_DIM)
-        width_b = 2 * ((b.size(-2) - 1) * b.stride(-2) + HEAD_DIM)
-        reach = max(a0 + width_a, b0 + width_b) - min(a0, b0)
-        nested = all(x >= 0 for x in rows) and (not rows or reach <= 2 * min(rows))
-        if nested and (a0 + width_a <= b0 or b0 + width_b <= a0):
-            return False
-    return True
+    return N.direct().may_overlap(a, b)
 
 
 def _dense_apart(t: torch.Tensor) -> bool:
     """True where no two elements of t share memory (expanded or overlapping windows do)."""
-    reach = 0
-    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
-        if s <= reach:
-            return False
-        reach += s * (n - 1)
-    return True
+    return N.direct().dense_apart(t)
 
 
 def _check_out(q, k, q_out, k_out) -> None:

@@ -56,3 +56,19 @@ def test_results_beside_the_inputs_or_in_the_place_of_q(native_built):
         assert got is out or got.data_ptr() == out.data_ptr()
         R.check_attention(got, None, ref)
     _native.device_check()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_in_place_of_a_batch_with_heads_in_front_of_tokens(native_built, interleaved):
+    from b200_attention_b200 import _native, ops
+
+    buf = rand(5, 3, 4 + 2 + 2, 50, 128)                                   # [batch, heads of q, k and v, tokens, 128]
+    q, k = buf[:, :4].transpose(1, 2), buf[:, 4:6].transpose(1, 2)
+    pos = torch.arange(50, device="cuda")
+    f = 10000.0 ** (-torch.arange(64, device="cuda", dtype=torch.float32) / 64)
+    want_q, want_k = ops.qk_norm_rope(q, k, pos, f, interleaved=interleaved)
+    v = buf[:, 6:].clone()
+    ops.qk_norm_rope(q, k, pos, f, interleaved=interleaved, out=(q, k))
+    torch.cuda.synchronize()
+    assert torch.equal(q, want_q) and torch.equal(k, want_k) and torch.equal(buf[:, 6:], v)
+    _native.device_check()
