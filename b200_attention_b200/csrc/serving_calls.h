@@ -223,6 +223,12 @@ inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, cons
     check_tokens("out of k", *given[1], &q);
     TORCH_CHECK(given[1]->sizes() == k->sizes(), "out of k must match k in shape");
   }
+  // q and k among one another: rotary.py
+  for (const at::Tensor* out : given) {
+    if (out == nullptr) continue;
+    for (const at::Tensor* read : {&positions, &inv_freq, weight[0], weight[1]})
+      TORCH_CHECK(read == nullptr || !may_overlap(*out, *read), "an output overlaps positions, inv_freq or a weight");
+  }
 
   c10::cuda::CUDAGuard guard(q.device());
   const at::Tensor qo = given[0] != nullptr ? *given[0] : empty_on(q.sizes(), at::kBFloat16, q.device());

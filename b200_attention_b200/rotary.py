@@ -67,7 +67,7 @@ def qk_norm_rope(
     positions: int32, int64 or fp32, [axes, tokens], or [axes, batch, tokens]; [tokens] for one axis. Without a
     batch axis a batch's entries share them. Angles are worked out in 64 bits: far positions lose nothing.
     q_weight, k_weight: [128], both bf16 or both fp32, or None (no norm). Inputs need strides that are multiples of 8
-    elements. `out`: tensors to write (may be q and k themselves). One rounding to bf16, at the end. A
+    elements. `out`: tensors to write (q and k themselves, or apart from all inputs). One rounding to bf16, at the end. A
     value that is not finite reaches the other one of its pair, or with a norm all of its head, and no further.
     Forward only.
     """

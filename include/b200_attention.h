@@ -262,7 +262,8 @@ B200ATTN_API int b200attn_forward_planned(const b200attn_planned_args* args);
  * pair j of y is turned by position[axis(j)] * inv_freq[j]: (a, b) -> (a cos - b sin, b cos + a sin). Pairs are
  * (j, j + 64), or (2j, 2j + 1) if interleaved. The first section[0] pairs take their position from axis 0, the
  * next section[1] from axis 1, and so on; pairs behind the last section are not turned. q_out and k_out may be
- * q and k themselves; otherwise they must not overlap them. */
+ * q and k themselves; otherwise they must not overlap them, and never positions, inv_freq, a weight or one another
+ * (not checked). */
 typedef struct b200attn_qk_norm_rope_args {
   uint32_t struct_bytes; /* sizeof(b200attn_qk_norm_rope_args), checked */
   int32_t batch, tokens, heads_q, heads_k, head_dim; /* heads_k may be 0 (k, k_out unused); head_dim 128 */

@@ -72,3 +72,27 @@ def test_rotation_in_place_of_a_batch_with_heads_in_front_of_tokens(native_built
     torch.cuda.synchronize()
     assert torch.equal(q, want_q) and torch.equal(k, want_k) and torch.equal(buf[:, 6:], v)
     _native.device_check()
+
+
+def test_rotated_rows_over_positions_frequencies_or_weights_are_refused(native_built):
+    from b200_attention_b200 import _native, ops
+
+    raw = torch.zeros(40 * 2 * 128 + 512, device="cuda", dtype=torch.bfloat16)
+    out = raw[:40 * 2 * 128].view(40, 2, 128)
+    before = raw.clone()
+    pos, f, w = torch.arange(40, device="cuda"), torch.ones(64, device="cuda"), rand(2, 128)
+    q = rand(1, 40, 2, 128)
+    bad = [
+        lambda: ops.qk_norm_rope(q, None, raw.view(torch.int64)[:40], f, out=(out, None)),
+        lambda: ops.qk_norm_rope(q, None, pos, raw.view(torch.float32)[64:128], out=(out, None)),
+        lambda: ops.qk_norm_rope(q, None, pos, f, q_weight=raw[256:384], out=(out, None)),
+        lambda: ops.qk_norm_rope(rand(3, 40, 2, 128), q, pos, f, k_weight=raw[256:384], out=(torch.empty_like(q), out)),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(RuntimeError, match="an output overlaps"):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    ops.qk_norm_rope(q, None, pos, raw[40 * 2 * 128:].view(torch.float32)[:64], q_weight=raw[-128:], out=(out, None))
+    torch.cuda.synchronize()
+    assert torch.equal(raw[40 * 2 * 128:], before[40 * 2 * 128:])
+    _native.device_check()
