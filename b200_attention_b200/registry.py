@@ -15,7 +15,7 @@ import hashlib
 from dataclasses import dataclass
 from pathlib import Path
 
-from . import _native
+from . import _native, build
 
 PKG = Path(__file__).resolve().parent
 HEAD_DIM = 128
@@ -73,13 +73,11 @@ def sha256_file(path: Path) -> str:
 
 
 def source_closure_sha256(spec: KernelSpec) -> str:
-    """Fingerprint of the kernel source and every header it includes (cf. registry.py:230-255)."""
+    """Fingerprint of the kernel source and every header it includes (cf. registry.py:230-255): all that the library
+    behind it is compiled from."""
     h = hashlib.sha256()
-    names = ["csrc/attn_fwd_sm100.cu", "csrc/capi.cu", "csrc/noalloc.cu", "csrc/attn_device_sm100.cuh",
-             "csrc/attn_kernels.cuh", "csrc/ptx_sm100.cuh", "csrc/host_common.cuh", "../include/b200_attention.h"]
-    for name in names:
-        p = (PKG / name).resolve()
-        h.update(name.encode())
+    for p in (*build.CORE_SOURCES, *build.CORE_HEADERS):
+        h.update(p.relative_to(PKG.parent).as_posix().encode())
         h.update(p.read_bytes())
     return h.hexdigest()
 
