@@ -4,6 +4,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAException.h>
@@ -24,11 +25,18 @@ inline void check_rc(int rc) {
               b200attn_last_error());
 }
 
-inline void check_bf16(const char* name, const at::Tensor& t) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (this library has no CPU path)");
-  TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16, got ", t.scalar_type());
+// These calls record nothing: neither for a backward pass nor along a forward-mode one (level 0 is the only one).
+inline void check_no_gradient(const char* name, const at::Tensor& t) {
   TORCH_CHECK(!(t.requires_grad() && c10::GradMode::is_enabled()), name,
               " requires grad: this library computes forward passes only");
+  TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()), name,
+              " carries a tangent: this library has no forward-mode gradients");
+}
+
+inline void check_bf16(const char* name, const at::Tensor& t) {
+  check_no_gradient(name, t);
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (this library has no CPU path)");
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16, name, " must be bfloat16, got ", t.scalar_type());
 }
 
 inline void check_rows(const char* name, const at::Tensor& t, int64_t heads, const at::Device& device) {
@@ -201,16 +209,15 @@ inline std::tuple<at::Tensor, at::Tensor> qk_norm_rope(const at::Tensor& q, cons
                   (pos.dim() == 3 && pos.size(0) == axes && pos.size(1) == batch && pos.size(2) == tokens),
               "positions must be [", axes, ", ", tokens, "] or [", axes, ", ", batch, ", ", tokens, "], got ",
               positions.sizes());
-  TORCH_CHECK(!((positions.requires_grad() || inv_freq.requires_grad()) && c10::GradMode::is_enabled()),
-              "positions or inv_freq requires grad: this library computes forward passes only");
+  check_no_gradient("positions", positions);
+  check_no_gradient("inv_freq", inv_freq);
   const at::Tensor* weight[2] = {q_weight.has_value() ? &*q_weight : nullptr, k_weight.has_value() ? &*k_weight : nullptr};
   for (const at::Tensor* w : weight) {
     if (w == nullptr) continue;
     TORCH_CHECK(w->device() == q.device() && w->dim() == 1 && w->size(0) == 128 && w->is_contiguous() &&
                     (w->scalar_type() == at::kBFloat16 || w->scalar_type() == at::kFloat),
                 "a weight must be a contiguous bf16 or fp32 vector of 128 on q's device");
-    TORCH_CHECK(!(w->requires_grad() && c10::GradMode::is_enabled()),
-                "a weight requires grad: this library computes forward passes only");
+    check_no_gradient("a weight", *w);
   }
   TORCH_CHECK(weight[0] == nullptr || weight[1] == nullptr || weight[0]->scalar_type() == weight[1]->scalar_type(),
               "q_weight and k_weight must have the same type");
