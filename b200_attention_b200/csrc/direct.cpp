@@ -117,7 +117,15 @@ PyObject* check_place(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+PyObject* free_tables(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  b200attn_torch::free_tables();
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"free_tables", &free_tables, METH_NOARGS, nullptr},
     {"may_overlap", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&may_overlap)), METH_FASTCALL, nullptr},
     {"same_place", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&same_place)), METH_FASTCALL, nullptr},
     {"dense_apart", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&dense_apart)), METH_FASTCALL, nullptr},

@@ -11,7 +11,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <atomic>
 #include <limits>
+#include <memory>
 #include <optional>
 #include <tuple>
 
@@ -65,6 +67,58 @@ inline bool capturing(cudaStream_t stream) {
   return status != cudaStreamCaptureStatusNone;
 }
 
+// A graph's replays read the table of the plan that its calls were captured with, whatever has become of the plan: the
+// graph owns a reference to it (a user object, which its executable form takes over) and gives it up when it is destroyed
+// and no replay runs any more. That happens on a thread of CUDA's, where neither CUDA nor Python may be called, so the
+// reference only goes to a list there; the next plan or call frees what is on it.
+struct GraphTable {
+  at::Tensor table;
+  GraphTable* next;
+};
+
+inline std::atomic<GraphTable*>& tables_given_up() {
+  static std::atomic<GraphTable*> list{nullptr};
+  return list;
+}
+
+inline void CUDART_CB give_up_table(void* held) {
+  GraphTable* t = static_cast<GraphTable*>(held);
+  t->next = tables_given_up().load(std::memory_order_relaxed);
+  while (!tables_given_up().compare_exchange_weak(t->next, t, std::memory_order_release, std::memory_order_relaxed)) {
+  }
+}
+
+// With the GIL held: the tensors may have Python's objects.
+inline void free_tables() {
+  if (tables_given_up().load(std::memory_order_relaxed) == nullptr) return;
+  for (GraphTable* t = tables_given_up().exchange(nullptr, std::memory_order_acquire); t != nullptr;) {
+    GraphTable* next = t->next;
+    delete t;
+    t = next;
+  }
+}
+
+// Before the call is captured, so that no graph holds a call without its table.
+inline void keep_for_graph(cudaStream_t stream, const at::Tensor& table) {
+  static unsigned long long last_capture = 0;  // of a capture's calls of one plan (one for each layer) the first does it
+  static const void* last_table = nullptr;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  cudaGraph_t graph = nullptr;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &status, &capture, &graph));
+  TORCH_CHECK(status == cudaStreamCaptureStatusActive && graph != nullptr, "the capture of this stream has failed");
+  if (capture == last_capture && table.const_data_ptr() == last_table) return;
+  cudaUserObject_t object = nullptr;
+  std::unique_ptr<GraphTable> held(new GraphTable{table, nullptr});
+  C10_CUDA_CHECK(cudaUserObjectCreate(&object, held.get(), give_up_table, 1, cudaUserObjectNoDestructorSync));
+  held.release();  // the object's now
+  const cudaError_t e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) (void)cudaUserObjectRelease(object, 1);
+  C10_CUDA_CHECK(e);
+  last_capture = capture;
+  last_table = table.const_data_ptr();
+}
+
 // A tensor that the caller gave as output: a backward pass that saved it must see that it has changed.
 inline void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -105,6 +159,10 @@ inline std::tuple<at::Tensor, at::Tensor, bool> attention_planned(const at::Tens
   c10::cuda::CUDAGuard guard(device);
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(device.index()).stream();
   const bool captured = capturing(stream);
+  if (captured)
+    keep_for_graph(stream, table);
+  else
+    free_tables();
   int64_t grid = plan[captured ? 8 : 5];
   const int64_t units = plan[captured ? 9 : 6], slots = plan[captured ? 10 : 7];
   if (k.size(0) == 0 && len_prefix == 0) grid = 0;  // no key for any replay to work on

@@ -82,10 +82,6 @@ class Schedule:
             lib.b200attn_plan_destroy(handle)
 
 
-# Tables that captured calls read: a graph does not keep the plan alive, and may be replayed without it.
-_tables_of_graphs: list = []
-
-
 class AttentionPlan:
     """Which CTA works on what, for sequences of the given lengths.
 
@@ -99,7 +95,8 @@ class AttentionPlan:
     replayed, so an updated plan changes what the replay does; `update` refuses lengths that a captured call has no
     room for. (What a replay does not compute, rows behind the new last sequence, keeps what the output held.) A plan
     may be used on any stream of its device, also by overlapping calls; only `update` must not overlap calls that use
-    it on other streams than the current one.
+    it on other streams than the current one. A graph keeps the table of its calls' plans for itself: it may be
+    replayed after the plan is gone, and gives the table back when it is destroyed.
     """
 
     def __init__(self, lens_q, lens_kv, *, heads: int, heads_kv: Optional[int] = None, causal: bool = True,
@@ -128,6 +125,7 @@ class AttentionPlan:
         self._put(s)
 
     def _new_table(self, s: Schedule) -> None:
+        N.direct().free_tables()
         self._table = torch.zeros(2 * s.table.numel() + 16384, dtype=torch.int32, device=self.device)
         self._table_stream = torch.cuda.current_stream(self.device).cuda_stream
 
@@ -146,8 +144,6 @@ class AttentionPlan:
                      i.wide_pieces)
 
     def _hold(self, rows_q: int, rows_kv: int) -> None:
-        if self._captured is None:
-            _tables_of_graphs.append(self._table)
         held = self._captured or (rows_q, rows_kv)
         self._captured = (min(held[0], rows_q), min(held[1], rows_kv))
 
