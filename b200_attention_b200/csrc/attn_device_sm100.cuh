@@ -131,7 +131,8 @@ __device__ __forceinline__ void issue_pv(uint32_t lead, uint32_t o_tmem, uint32_
 // ------------------------------------------------------------------------------------------
 // Softmax arithmetic: one query row per thread
 // ------------------------------------------------------------------------------------------
-// Keys at or beyond `valid` (0 < valid < 128) do not exist: push their scores to -inf.
+// Keys at or beyond `valid` are masked: push their scores to -inf. Any `valid` will do: none of the tile's keys is left
+// where it is 0 or less, all of them where it is 128 or more.
 __device__ __forceinline__ void mask_tail(uint32_t (&s)[4][32], int valid) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
