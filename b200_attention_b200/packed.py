@@ -167,12 +167,25 @@ class AttentionPlan:
         self._put(s)
 
 
+def used_on(stream: torch.cuda.Stream, *tensors) -> None:
+    """What a call on a given stream reads or writes may be freed before it has run: its memory goes to nobody else until
+    then. (A captured call's tensors are the caller's to keep, as with any captured call.)"""
+    with torch.cuda.stream(stream):
+        if torch.cuda.is_current_stream_capturing():
+            return
+    for t in tensors:
+        if t is not None:
+            t.record_stream(stream)
+
+
 def _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, stream):
     if stream is not None and stream != torch.cuda.current_stream(plan.device):
         if stream.device != plan.device:
             raise RuntimeError(f"stream is on {stream.device}, the plan on {plan.device}")
         with torch.cuda.stream(stream):
-            return _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
+            result = _run(q, k, v, k_prefix, v_prefix, plan, softmax_scale, return_lse, out, None)
+        used_on(stream, q, k, v, k_prefix, v_prefix, out)
+        return result
     o, lse, captured = (N._direct or N.direct()).attention_planned(q, k, v, k_prefix, v_prefix, plan._table, plan._now,
                                                                    softmax_scale, return_lse, out)
     if captured:
@@ -190,7 +203,8 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: At
     (natural log). A token that sees no key gets O = 0 and LSE = -inf. Rows of q behind the plan's last sequence are
     not read; their rows of a given `out` keep what they hold, in an O made here they are 0 (LSE: -inf). Rows of
     k and v outside the plan's sequences have no influence, whatever they hold. `out` may be q itself, and otherwise
-    must not overlap q, k, v or a prefix, nor itself.
+    must not overlap q, k, v or a prefix, nor itself. `stream`: where to launch instead of the current stream; what the
+    call reads has to be there by that stream's order, and may be let go of once the call has returned.
     Forward only. softmax_scale <= 0: 1 / sqrt(128).
     """
     if not isinstance(plan, AttentionPlan):

@@ -8,6 +8,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _native as N
+from .packed import used_on
 
 def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
     return N.direct().same_place(a, b)
@@ -69,6 +70,8 @@ def qk_norm_rope(
     q_weight, k_weight: [128], both bf16 or both fp32, or None (no norm). Inputs need strides that are multiples of 8
     elements. `out`: tensors to write (q and k themselves, or apart from all inputs). One rounding to bf16, at the end. A
     value that is not finite reaches the other one of its pair, or with a norm all of its head, and no further.
+    `stream`: where to launch instead of the current stream; what the call reads has to be there by that stream's order,
+    and may be let go of once the call has returned.
     Forward only.
     """
     if sections is None:
@@ -83,7 +86,9 @@ def qk_norm_rope(
         if stream.device != q.device:
             raise RuntimeError(f"stream is on {stream.device}, q on {q.device}")
         with torch.cuda.stream(stream):
-            return _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out)
+            result = _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out)
+        used_on(stream, q, k, positions, inv_freq, q_weight, k_weight, q_out, k_out if k is not None else None)
+        return result
     return _launch(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, interleaved, q_out, k_out)
 
 
