@@ -27,11 +27,13 @@
 //
 // Measured on a B200 (calls back to back; a plain copy reaches 6.4 TB/s, a cuBLAS bf16 product 1658 TFLOPS in a burst and
 // 1400 under the power cap):
-//   one prompt of 16384 tokens, 16 heads, causal    0.86 ms in a burst (1280 TFLOPS), 0.99 ms under the power cap (1110);
-//       1.46 M cycles, tensor pipe busy 63 % of them: bound by the chain, as attn_fwd_ws_kernel (1.45 M) is
-//   64 single tokens, 32 + 8 heads, 100-12000 keys  0.23 ms, 6.1 TB/s: bound by memory
-//   64 tokens behind 32768 shared rows, 32 + 8 heads, up to 1024 keys of their own    70 us, 3.8 TB/s: half the CTAs
-//       work on the prefix (chain), half on short runs of keys that each start anew (see NotedWait)
+//   one prompt of 16384 tokens, 16 heads, causal    0.84 ms in a burst (1300 TFLOPS), 0.99 ms under the power cap (1110);
+//       1.47 M cycles, tensor pipe busy 62 % of them: bound by the chain, as attn_fwd_ws_kernel (1.45 M) is
+//   64 single tokens, 32 + 8 heads, 100-12000 keys  0.23 to 0.25 ms from GPU to GPU in a burst (5.6 to 6.1 TB/s), 0.26 for
+//       long (5.3): bound by memory
+//   64 tokens behind 32768 shared rows, 32 + 8 heads, up to 1024 keys of their own    72 to 81 us, 3.3 to 3.7 TB/s: half
+//       the CTAs work on the prefix (chain), half on short runs of keys, which each have a start, a hand-over and a partial
+//       result of their own
 //   one token, 128 keys                             5 us: load, scores, softmax, product, store one after the other
 // Asked for and not kept, being slower: K/V tiles prefetched into the L2 two to six ahead (single tokens 235 -> 289 us and
 // more), a third slot in the K/V ring for CTAs of small pieces (228 -> 232 us), boxes of 32 rows for the tile in which a
@@ -94,13 +96,15 @@ static_assert(kPlanSmemBytes <= 227 * 1024, "shared memory of a CTA");
 
 // Waits of short code: one loop, and a timeout is noted in shared memory (from the abort flag on), for the CTA to report
 // when it ends. For launches without pieces of two Q tiles. There a round of two short pieces runs through more code than
-// an SM's instruction cache holds (150 lines are fetched for each piece of one K/V tile, 10 for a further tile), the
+// an SM's instruction cache holds (137 requests to the GPC's cache for each piece of one K/V tile, 33 for a second tile), the
 // caches behind it serve the SMs of a GPC together, and CTAs in larger GPCs take longer for the same work (148 tokens of
 // 128 keys: 17 us with 12 SMs to a GPC, 25 us with 20). With these waits in the place of WaitCtx's:
-//   148 tokens, 32 + 8 heads, of 128 / 256 / 300 keys   28.9 / 38.8 / 51.1 -> 26.6 / 36.0 / 49.0 us
-//   100 tokens of 5-600 keys                            37.6 -> 36.0 us
-//   64 tokens of 100-12000 keys                         233 -> 231 us
-// Prompts are 2 to 4 % slower with them. Scores taken 32 at a time in a loop (half the code of a tile) cost 6 % at 64
+//   148 tokens, 32 + 8 heads, of 128 / 256 / 300 keys   29.0 / 38.7 / 49.9 -> 27.4 / 35.4 / 47.1 us
+//   100 tokens of 5-600 keys                            44.8 -> 42.4 us
+//   64 tokens of 100-12000 keys                         238 -> 236 us
+// Prompts are 3 to 6 % slower with them (16384 tokens, 16 heads: 956 -> 1013 us). WaitCtx's build spills 24 bytes a
+// thread, which are loaded 368 bytes' worth; without its constants in registers that falls to 76 and prompts take 1 to
+// 3 % longer. Scores taken 32 at a time in a loop (half the code of a tile) cost 6 % at 64
 // tokens of 100-12000 keys, MMAs issued in loops 2 %.
 struct NotedWait : WaitCtx {
   __device__ __forceinline__ void note(int site, uint32_t parity) const {
@@ -630,9 +634,10 @@ __device__ __forceinline__ void store_result(const PlanParams& p, const PlanPiec
 // and go the exact way where the tile's sum says that it has to move. The maximum comes first because the largest
 // probability of a row is then 2^0 = 1 and loses nothing when it is rounded to bf16: where one key of the first tile
 // outweighs the others (its score 9 to 15, theirs about N(0, 1)) a reference of 0 rounds all of the row's result once
-// more, by up to 2^-8 (error against 64 bits 0.0021 -> 0.0013 of the norm at 128 keys, 0.0024 -> 0.0017 at 1024), and
-// with a few keys so it does for any scores. It costs a part of one tile's time per piece: 148 tokens of 128 keys 26.2
-// -> 27.3 us, of 256 34.5 -> 35.3, of 300 46.2 -> 46.9, 64 of 100-2000 53.1 -> 53.4, whole prompts within 1 %.
+// more, by up to 2^-8 (error against 64 bits, of the norm: single tokens of 128 keys 0.0021 -> 0.0013, of 1024 0.0024 ->
+// 0.0016, of 4096 0.0024 -> 0.0017, prompts of 1024 0.0021 -> 0.0015), and with a few keys it does so for any scores. It
+// costs a part of one tile's time per piece: 148 tokens of 128 keys 26.2 -> 27.3 us, of 256 34.5 -> 35.3, of 300 46.2 ->
+// 46.9, 64 of 100-2000 53.1 -> 53.4, 64 of 100-12000 230 either way, whole prompts no more (16384 tokens 850 -> 843).
 // One difference: rows that see no key of a tile, or of the whole piece. Their m becomes -inf, which sends them down the
 // exact path, where it is subtracted as 0 so that every probability is 2^-inf = 0.
 template <class Wait>

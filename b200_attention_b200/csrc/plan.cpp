@@ -24,9 +24,10 @@ constexpr int kTile = 128;
 // A piece of one Q tile runs on one of a CTA's two lanes: alone it is bound by its chain of steps, beside another lane
 // by what the two share, which is above all memory (64 KB per tile). Next to a prefix, whose pieces load memory on
 // every CTA, a tile costs more of that; without one a CTA that has more tiles than others gets more of the memory's
-// rate, and a piece's start weighs more. One pair of figures for both costs a tenth of the time on one side or the
-// other (10 tokens of 4000 keys, 40 heads: 48.8 us with the first, 41.1 with the second; 90 tokens on a prefix of
-// 3000: 41.0 and 45.4).
+// rate, and a piece's start weighs more. Two pairs of figures are worth little on average and much at some shapes: over
+// 26 decode and prefix shapes, measured twice, 2.0 and 1.1 % in the mean, from -16 % (10 tokens of 4000 keys, 40 heads:
+// 48.8 us with the first pair everywhere, 41.1 as it is) to +6 % (16 tokens of 1000-8000 keys: 49.2 -> 52.2); the second
+// pair everywhere costs 90 tokens on a prefix of 3000 41.0 -> 45.4 us.
 constexpr int64_t kTilePair = 1000;
 constexpr int64_t kTilePairPrefix = 1250;  // the same, with every CTA on keys of its own, which come from memory
 constexpr int64_t kPairStart = 2200;    // Q load, first scores, last PV, stores

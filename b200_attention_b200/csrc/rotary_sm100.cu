@@ -43,6 +43,9 @@ constexpr int kPairs = 64;
 //   65536 tokens x 24 heads (6)                      155.2               147.6               155.7
 //   1537 tokens x 24 heads, 2 warps a token (3)        6.8                 6.9                 6.2
 //   32 tokens x 40 heads, 10 warps a token (1)         4.0                 3.7                 3.6
+// One warp a token, 16384 and 65536 tokens, both pairings, 8 to 64 heads: the second is 3 to 20 % faster at 8, 12, 16, 20
+// and 24 heads, the first 1 to 6 % at 26, 28, 30, 32, 36, 40, 48 and 64 (65536 tokens x 32 heads, half-split: level).
+// ptxas spills 68, 48 and 8 bytes a thread in the three variants.
 constexpr int kFewHeads = 24;  // of a token in one warp
 
 __device__ __forceinline__ f2 f2_mul(f2 a, f2 b) {
