@@ -16,9 +16,11 @@ def overwritten_behind(call, stream, make):
     """`call(*make())` on a stream that is busy, its inputs freed at once and their sizes allocated and filled anew."""
     torch.cuda.synchronize()
     tensors = make()
+    for t in tensors:
+        torch.zeros(1, dtype=t.dtype, device="cuda")  # the kernels that fill are loaded
     torch.cuda.synchronize()
     with torch.cuda.stream(stream):
-        torch.cuda._sleep(100_000_000)
+        torch.cuda._sleep(400_000_000)
     got = call(*tensors)
     shapes = [(t.shape, t.dtype) for t in tensors]
     places = {t.data_ptr() for t in tensors}
